@@ -283,6 +283,64 @@ KLAB_API int klab_decode_attention(const void* q, const void* k_new, const void*
                                    const int* len_ptr, int len, int max_len, int heads, int kv_heads, float scale,
                                    void* stream);
 
+/* ---- A batch of requests over 4-bit K/V pages.
+ *
+ * pages: uint8 [num_pages, kv_heads, page_size * dim * 9 / 8], 16-byte aligned; page_size 16, 32, .. 1024 (a power of
+ * two), dim 64, 128 or 256, num_pages * page_size < 2^31. A value is (code - 8) * scale with one FP16 scale per 32 dims of
+ * a token and head: scale = RN16(min(max|x| / 7, 65504)), code = clamp(RNE(x / scale), -7, 7) + 8 (8 where scale is 0
+ * or x is NaN). slot = page * page_size + offset names a token's place; table[requests, width] holds the pages of each
+ * request in order. No counterpart in the reference, whose cache is one sequence's (research/l2-prefetch/src/
+ * decode_attn.py:20-107). */
+
+/* Results of klab_kv_build_step. */
+#define KLAB_STEP_OK 0
+#define KLAB_STEP_LENGTH 1 /* a negative length or new-token count */
+#define KLAB_STEP_TABLE 2  /* a request needs more pages than the table has columns */
+#define KLAB_STEP_PAGES 3  /* not enough free pages */
+#define KLAB_STEP_TOKENS 4 /* more new tokens than max_tokens */
+
+/* One step of a batch: request i (of `requests` <= 8192) with lengths[i] cached tokens adds new_tokens[i]. New pages come
+ * from the top of free_pages[0 .. free_count) (requests in order, pages in order) and go into table in place. Writes for
+ * each new token x (requests in order) slots[x], positions[x] and rows[x] (its request; -1, 0, -1 for max_tokens > x >=
+ * the step's tokens), starts[requests + 1] (each request's first token), lengths_out[i], free_count_out and *result. A
+ * result other than KLAB_STEP_OK means that nothing was given out: no tokens, lengths and count as they were, table
+ * untouched, device status 5. lengths_out and free_count_out may be lengths and free_count (update in place), no other
+ * output may overlap an input. A page out of range gives slot -1 and device status 4. */
+KLAB_API int klab_kv_build_step(const int* new_tokens, const int* lengths, int* table, const int* free_pages,
+                                const int* free_count, int requests, int width, int num_pages, int page_size,
+                                int max_tokens, int* slots, int* positions, int* rows, int* starts, int* lengths_out,
+                                int* free_count_out, int* result, void* stream);
+/* Requests with ended[i] != 0 give their pages back: pushed on free_pages[*free_count ..) (requests in order, pages in
+ * order), table entries -1, lengths 0, all in place. Nothing happens (device status 4) when a page of theirs or the count
+ * is out of range. */
+KLAB_API int klab_kv_release(const unsigned char* ended, int* lengths, int* table, int* free_pages, int* free_count,
+                             int requests, int width, int num_pages, int page_size, void* stream);
+/* Byte offset from `pages` of the 16-token block of `slot` and kv head `head`; -1 when they lie outside (host only). */
+KLAB_API long long klab_kv_block_offset(int slot, int head, int num_pages, int kv_heads, int page_size, int dim);
+/* Rows k, v [tokens, kv_heads, dim] (BF16 or FP16; strides in elements between tokens and heads, multiples of 4; 8-byte
+ * aligned) into the pages at slots[token]; slot -1 is skipped, another slot outside the pages too (device status 4). Two
+ * tokens of one call must not name the same slot. */
+KLAB_API int klab_kv_store(const void* k, const void* v, int dtype, long long k_stride, long long v_stride,
+                           long long k_head, long long v_head, void* pages, const int* slots, int tokens, int num_pages,
+                           int page_size, int kv_heads, int dim, void* stream);
+/* The rows at slots[token] as k_out, v_out [tokens, kv_heads, dim] in `dtype` (each value rounded once; FP32 is exact);
+ * zeros for slot -1 and for one outside the pages (device status 4). */
+KLAB_API int klab_kv_read(const void* pages, const int* slots, void* k_out, void* v_out, int dtype, int tokens,
+                          int num_pages, int page_size, int kv_heads, int dim, void* stream);
+/* Attention over the pages: q[tokens, heads, dim] (BF16 or FP16, q_stride elements between tokens, a multiple of 8; q and
+ * out 16-byte aligned) with request i's tokens at starts[i] .. starts[i + 1) (at most max_new <= 16 each, the last ones of
+ * its lengths[i] tokens): token j of n sees positions below lengths[i] - n + j + 1, a row that sees none gives 0. out
+ * [tokens, heads, dim]; rows of no request are left as they were. heads / kv_heads <= 64. scratch:
+ * klab_kv_attention_scratch bytes (a negative value there is an error code), of any content, for this call alone. Lengths
+ * and starts that make no sense leave the request's rows as they were (device status 3); a table entry that is no page
+ * counts as 16-token blocks that nobody sees (device status 4). */
+KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
+                               const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
+                               int tokens, int requests, int width, int num_pages, int page_size, int heads,
+                               int kv_heads, int dim, int max_new, float scale, void* stream);
+KLAB_API long long klab_kv_attention_scratch(int requests, int width, int page_size, int heads, int kv_heads, int dim,
+                                             int max_new);
+
 /* Fused: the projection out[M,N] = xn . W^T (BF16 W [N,K], BF16 out) with xn computed while
  * x is staged, as klab_add_rmsnorm would (x_out, when not null, gets RNE(res + y)); bit-identical
  * to klab_add_rmsnorm followed by klab_raw_linear. K % 8 == 0. x_out and out must not overlap res,
@@ -392,8 +450,9 @@ KLAB_API int klab_l2_prefetch(const void* p, long long bytes, int blocks, int th
 KLAB_API int klab_set_option(int option, int value);
 KLAB_API int klab_get_option(int option);
 /* Read the current device's status word (0 = no device-side error; 1 = a bulk copy wait gave up,
- * 2 = a peer flag wait gave up, 3 = a length read from device memory was out of range); clear it
- * when clear != 0. */
+ * 2 = a peer flag wait gave up, 3 = a length read from device memory was out of range, 4 = a page,
+ * slot or table entry was, 5 = a batch step was refused, 6 = an adapter index was out of range); clear it when
+ * clear != 0. */
 KLAB_API int klab_device_status(int clear);
 KLAB_API const char* klab_error_string(int code);
 KLAB_API int klab_version(void);

@@ -56,6 +56,13 @@ _SIGNATURES = {
     "klab_silu_mul": (_I, [_P, _P, _I, _I, _P]),
     "klab_decode_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, ct.c_longlong, _P, _P, _I, _I, _I, _I, ct.c_float,
                                     _P]),
+    "klab_kv_build_step": (_I, [_P] * 5 + [_I] * 5 + [_P] * 8),
+    "klab_kv_release": (_I, [_P] * 5 + [_I] * 4 + [_P]),
+    "klab_kv_block_offset": (ct.c_longlong, [_I] * 6),
+    "klab_kv_store": (_I, [_P, _P, _I] + [ct.c_longlong] * 4 + [_P, _P] + [_I] * 5 + [_P]),
+    "klab_kv_read": (_I, [_P] * 4 + [_I] * 6 + [_P]),
+    "klab_kv_attention": (_I, [_P, ct.c_longlong, _I] + [_P] * 6 + [ct.c_longlong] + [_I] * 9 + [ct.c_float, _P]),
+    "klab_kv_attention_scratch": (ct.c_longlong, [_I] * 7),
     "klab_add_rmsnorm_linear": (_I, [_P, _P, _P, ct.c_float, _P, _P, _P, _I, _I, _I, _P, _SZ, _P]),
     "klab_silu_mul_linear": (_I, [_P, _P, _P, _I, _I, _I, _P, _SZ, _P]),
     "klab_int8_linear": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _SZ, _P]),

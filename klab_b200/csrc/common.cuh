@@ -20,6 +20,9 @@ enum DeviceStatus : int {
   kStatusMbarTimeout = 1,     // a bulk copy did not complete within the limit
   kStatusFlagTimeout = 2,     // a peer flag was not raised within the limit
   kStatusBadLength = 3,       // a length read from device memory was out of range
+  kStatusBadPage = 4,         // a page, slot or table entry read from device memory was out of range
+  kStatusStepRefused = 5,     // a batch step asked for more pages, tokens or table columns than there are
+  kStatusBadAdapter = 6,      // an adapter index read from device memory was out of range
 };
 
 // Iteration limit for every spin on an mbarrier or a flag. try_wait suspends for a

@@ -2,30 +2,35 @@
 // out = sum_p softmax_p(scale * q . K_p) V_p over the positions p < length_i - new_i + j + 1, grouped query heads, ragged
 // lengths read from device memory. Stands beside the single-sequence BF16 attention of decode_attn.cu.
 //
-// Work: an item is (request, tile of rows, run of 16-token blocks); CTA (item, kv head) has 4 warps that take the run's
-// blocks in turn. The rows of a kv head are its query heads times the request's new tokens, in tiles of 8 or 16. The run
-// length comes from the lengths themselves (every CTA adds up all requests), so uneven batches and single long ones fill
-// the machine alike; a run that is not the whole request leaves its sums in scratch, and combine_kernel joins them in the
-// order of the runs (a second launch, because per-call scratch then needs no zeroed counters: two captured graphs or two
-// streams never share any).
+// Work: a segment is a tile of 8 query rows of a request and kv head (its query heads times its new tokens), in units of
+// 32 tokens. All segments of a kv head, one behind the other, are cut into equal shares, one for each CTA that the machine
+// holds at once; every CTA adds up all requests to find its own, so uneven batches and single long ones fill the machine
+// alike, and its 4 warps take a piece's units in turn. A piece that is not a whole segment leaves its sums in scratch, and
+// kv_combine_kernel joins them in order (a second launch, because per-call scratch then needs no zeroed counters: two
+// captured graphs or two streams never share any). Tables of at most 512 tokens a request are not cut: whole segments are
+// dealt, and the second launch is saved.
 //
-// Per block and warp (K and V codes and scales: one bulk copy of 18 * D bytes into the warp's ring):
+// Per unit and warp (two blocks of 16 tokens: K and V codes and scales, one bulk copy of 18 * D bytes each into the
+// warp's ring):
 //   S^T = K Q^T   mma.m16n8k16, A = 16 tokens x 16 dims of codes u as FP16 subnormals (u * 2^-24, exact), B = q in FP16
-//                 times a power of two (its row's maximum near 2^10, so nothing that counts is lost); the accumulator starts
-//                 at -8 * 2^-24 * sum q of the group, which turns u into u - 8 without an instruction, and is multiplied
-//                 by the token's FP32 scale after each group of 32 dims.
-//   softmax       in base 2 against a reference exponent `ref` of the row that moves only when a score passes it by 2^4,
-//                 so most blocks need no rescale and no cross-lane maximum; sums in FP32.
+//                 times a power of two (its row's maximum in [2^14, 2^15), so nothing that counts is lost); each group of
+//                 32 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
+//                 more MMA of the scales with the groups' sums of q in two FP16 terms, and starts the sum.
+//   softmax       in base 2 against a reference `ref` of the row that moves only when a score passes it by 2^14, so most
+//                 units need no rescale and no cross-lane maximum; sums in FP32.
 //   O^T += V^T P' A = 16 dims x 16 tokens of codes (FP16 subnormals), B = P' = p * (V scale of the token and group) in
-//                 FP16. `ref` holds P' between 2^-16 and 2^15 with room below for the tail (FP16 subnormals end 2^-32
-//                 under the row's largest weight), so the rounding of p and of the product, 2^-11 relative each at most, is
-//                 what the FP16 operand costs. sum P' of a group comes from an MMA with ones, and -8 * sum P' turns u into
-//                 u - 8 at the end.
+//                 FP16, below 2^15 with room under it for the tail (FP16 subnormals end 2^-34 under the row's largest
+//                 weight at scales near 1). For BF16 outputs p and the product are rounded to FP16 in turn (2^-11 relative
+//                 each at most: 3 * 10^-4 of the result in the mean, a fifth of BF16's own 1.7 * 10^-3); for FP16 outputs
+//                 the product is formed in FP32 and rounded once (both roundings would show beside FP16's 2 * 10^-4; it
+//                 costs 6 %). sum P' of each group comes from an MMA with ones, and -8 sum P' turns u into u - 8 at the
+//                 end, so u and 8 meet the same P' and a code of 8 stays an exact 0. (One MMA of the scales with p in place
+//                 of the four with ones saved 1.5 % and lost that.)
 // Scores beyond a row's last position are -inf before the softmax, and the scales of tokens beyond the request are zeroed,
 // so whatever the allocator left there (NaN scales included) has no part.
 //
-// What bounds it: HBM for long caches (4.5 bits a value; about 13 instructions a lane per 8 K and 8 V values keep the
-// issue slots near half), launch and dependent loads (lengths, table, first block) for short ones.
+// What bounds it: long caches the issue slots (about 470 instructions a warp and unit of 4608 bytes at D = 128, IPC 2.3),
+// before HBM; short ones launch and dependent loads (lengths, table, first block).
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -42,25 +47,31 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 8;  // query rows of a tile (the MMA's N)
 #ifndef KLAB_KV_SLOTS
-#define KLAB_KV_SLOTS 4  // blocks in flight per warp
+#define KLAB_KV_SLOTS 2  // units of two blocks that a warp's ring holds
 #endif
 constexpr int kSlots = KLAB_KV_SLOTS;
-#ifndef KLAB_KV_MIN_RUN
-#define KLAB_KV_MIN_RUN 8  // blocks a run has at least (two per warp)
+#ifndef KLAB_KV_MIN_SHARE
+#define KLAB_KV_MIN_SHARE 4  // units a CTA takes at least
 #endif
-constexpr int kMinRun = KLAB_KV_MIN_RUN;
-#ifndef KLAB_KV_CTAS_PER_SM
-#define KLAB_KV_CTAS_PER_SM 8  // CTAs per SM that the run length aims at
+constexpr int kMinShare = KLAB_KV_MIN_SHARE;
+constexpr int kUnitTokens = 2 * kKvBlock;
+#ifndef KLAB_KV_WHOLE
+#define KLAB_KV_WHOLE 16
 #endif
+constexpr int kWholeUnits = KLAB_KV_WHOLE;
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kSlack = 4.0f;  // log2 of how far a score may pass the row's reference before it moves
+// A row's weights are 2^(score - ref) with ref = (a score near the largest) - 10, moved when a score passes it by 2^14; V
+// scales below 2 then keep P' below 2^15.
+constexpr float kRefBelow = 10.0f, kMoveAt = 14.0f;
 
-struct RunHeader {
-  int run, runs;   // this run, and how many the (request, tile) has; runs = 0: nothing here
-  int rows;        // rows of the tile
-  int row0;        // its first row within the request: token row0 / group, head row0 % group
-  int token0;      // the request's first token
+// Of each CTA: where its share begins inside a segment (a tile of rows of a request), what the CTAs from `first` to `last`
+// of that segment left in scratch has to be joined.
+struct Header {
+  int first, last;  // last = -1: nothing to join
+  int rows, row0;   // rows of the tile, its first row within the request: token row0 / group, head row0 % group
+  int token0;       // the request's first token
   int pad[3];
 };
 
@@ -71,12 +82,12 @@ struct KvAttnParams {
   const int* lengths;
   const int* starts;
   unsigned short* out;
-  RunHeader* headers;
-  float2* stats;   // [item][kv head][row] (ref, sum)
-  float* sums;     // [item][kv head][row][dim]
+  Header* headers;  // [CTA of a kv head]
+  float2* stats;    // [CTA of a kv head][kv head][2][row] (ref, sum): records of the CTA's first and last piece
+  float* sums;      // [..][dim]
   int* status;
   long long q_stride;
-  int requests, tokens, width, num_pages, page_shift, heads, kv_heads, group, max_new, target;
+  int requests, tokens, width, num_pages, page_shift, heads, kv_heads, group, group_div, max_new, max_length, whole;
   float scale_log2e;
 };
 
@@ -119,6 +130,9 @@ __device__ __forceinline__ unsigned max_h2(unsigned a, unsigned b) {
   return r;
 }
 
+__device__ __forceinline__ float lo_f32(unsigned w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float hi_f32(unsigned w) { return __high2float(*reinterpret_cast<const __half2*>(&w)); }
+
 template <int N>
 __device__ __forceinline__ void lds_words(unsigned addr, unsigned (&w)[N]) {
   static_assert(N == 1 || N == 2 || N == 4 || N == 8, "words of one run");
@@ -135,184 +149,230 @@ __device__ __forceinline__ void lds_words(unsigned addr, unsigned (&w)[N]) {
   }
 }
 
-// Requests are handed to CTAs by adding up all of them; a request whose lengths make no sense counts nothing.
+// row / group for row < 1024 and group <= 64 (div = ceil(2^16 / group): exact while row * (group - 1) < 2^16).
+__device__ __forceinline__ int by_group(const KvAttnParams& p, int row) { return (row * p.group_div) >> 16; }
+
+// A request as the lengths say; tiles = 0 for one without new tokens or whose numbers make no sense.
 struct Request {
-  int length, fresh, token0;
-  bool valid, bad;
+  int length, fresh, token0, tiles, units;
 };
 
-__device__ __forceinline__ Request load_request(const KvAttnParams& p, int i) {
+__device__ __forceinline__ Request make_request(const KvAttnParams& p, int length, int start, int end, bool& bad) {
   Request r;
-  r.length = p.lengths[i];
-  r.token0 = p.starts[i];
-  r.fresh = p.starts[i + 1] - r.token0;
-  r.bad = r.fresh < 0 || r.fresh > p.max_new || r.token0 < 0 || r.token0 > p.tokens - max(r.fresh, 0) || r.length < 0 ||
-          (static_cast<long long>(r.length) + (1 << p.page_shift) - 1) >> p.page_shift > p.width;
-  r.valid = !r.bad && r.fresh > 0;
+  r.length = length;
+  r.token0 = start;
+  r.fresh = end - start;
+  const bool wrong =
+      start < 0 || end < start || end > p.tokens || r.fresh > p.max_new || length < 0 || length > p.max_length;
+  bad |= wrong;
+  r.tiles = wrong ? 0 : (r.fresh * p.group + kRows - 1) / kRows;
+  // A request without a token has a unit that sees nothing; segments that are dealt whole count one unit each.
+  r.units = length > 0 && !p.whole ? (length - 1) / kUnitTokens + 1 : 1;
   return r;
 }
 
-__device__ __forceinline__ int blocks_of(int length) { return length > 0 ? (length - 1) / kKvBlock + 1 : 1; }
+// Units of all (request, tile) one behind the other, requests in order; a CTA takes `share` of them from `pos` on. Every
+// warp works its piece out for itself: the loads are the same few lines for the whole machine, and no barrier is needed.
+struct Share {
+  int pos, end, share;       // this CTA's units
+  int request, tile, unit;   // the segment that holds `pos`, and the unit within it
+  Request r;
+};
 
-// Sum over the CTA's threads of v, and the exclusive prefix of this thread in `before`. Two barriers.
-__device__ __forceinline__ long long cta_scan(long long v, long long* parts, long long& before) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long s = v;
+__device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int ctas, bool report) {
+  constexpr int kEach = 4;  // requests per lane and pass
+  const int lane = threadIdx.x & 31;
+  Request r[kEach];
+  bool bad = false;
+  auto load = [&](int base) {
+    int length[kEach] = {}, start[kEach] = {}, end[kEach] = {};
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, s, d);
-    if (lane >= d) s += up;
-  }
-  if (lane == 31) parts[warp] = s;
-  __syncthreads();
-  long long total = 0, base = 0;
+    for (int j = 0; j < kEach; ++j) {
+      const int i = base + 32 * j + lane;
+      if (base + 32 * j < p.requests && i < p.requests) {
+        length[j] = __ldg(p.lengths + i);
+        start[j] = __ldg(p.starts + i);
+        end[j] = __ldg(p.starts + i + 1);
+      }
+    }
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) base += parts[w];
-    total += parts[w];
+    for (int j = 0; j < kEach; ++j) r[j] = make_request(p, length[j], start[j], end[j], bad);
+  };
+  int all = 0;
+  for (int base = 0; base < p.requests; base += 32 * kEach) {
+    load(base);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) all += r[j].tiles * r[j].units;
   }
-  __syncthreads();
-  before = base + s - v;
-  return total;
+  all = __reduce_add_sync(0xffffffffu, all);
+  if (bad && report) record_status(p.status, kStatusBadLength);
+  Share it;
+  it.share = max(p.whole ? 1 : kMinShare, (all + ctas - 1) / ctas);
+  it.pos = min(static_cast<long long>(cta) * it.share, static_cast<long long>(all));
+  it.end = min(it.pos + it.share, all);
+  it.request = it.tile = it.unit = it.r.tiles = 0;
+  if (it.pos >= it.end) return it;
+  int carry = 0;
+  for (int base = 0; base < p.requests; base += 32 * kEach) {
+    if (p.requests > 32 * kEach) load(base);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (base + 32 * j < p.requests && it.r.tiles == 0) {
+        const int mine = r[j].tiles * r[j].units;
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += up;
+        }
+        const int at = it.pos - carry - (upto - mine);
+        const unsigned owner = __ballot_sync(0xffffffffu, at >= 0 && at < mine);
+        if (owner) {
+          const int from = __ffs(owner) - 1;
+          it.request = base + 32 * j + from;
+          it.r.length = __shfl_sync(0xffffffffu, r[j].length, from);
+          it.r.fresh = __shfl_sync(0xffffffffu, r[j].fresh, from);
+          it.r.token0 = __shfl_sync(0xffffffffu, r[j].token0, from);
+          it.r.tiles = __shfl_sync(0xffffffffu, r[j].tiles, from);
+          it.r.units = __shfl_sync(0xffffffffu, r[j].units, from);
+          const int in_request = __shfl_sync(0xffffffffu, at, from);
+          it.tile = in_request / it.r.units;
+          it.unit = in_request - it.tile * it.r.units;
+        }
+        carry += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (it.r.tiles) break;
+  }
+  return it;
 }
 
-template <int NG, int NT, bool kBf16>
-__global__ void __launch_bounds__(kThreads) kv_attn_kernel(const KvAttnParams p) {
-  constexpr int D = 32 * NG, Q = NG < 4 ? NG : 4, NQ = NG / Q, ROWS = 8 * NT;
+// The segment behind this one (there is one while pos < end).
+__device__ __forceinline__ void next_segment(const KvAttnParams& p, Share& it) {
+  it.unit = 0;
+  if (++it.tile < it.r.tiles) return;
+  it.tile = 0;
+  bool bad = false;
+  do {
+    ++it.request;
+    it.r = make_request(p, __ldg(p.lengths + it.request), __ldg(p.starts + it.request),
+                              __ldg(p.starts + it.request + 1), bad);
+  } while (it.r.tiles == 0 && it.request + 1 < p.requests);
+}
+
+#ifndef KLAB_KV_RESIDENT
+#define KLAB_KV_RESIDENT 3
+#endif
+// CTAs per SM the registers are cut for.
+constexpr int kv_resident(int ng) { return ng <= 4 ? KLAB_KV_RESIDENT : 2; }
+
+__device__ __forceinline__ long long record_of(const KvAttnParams& p, int cta, int kvh, int which) {
+  return ((static_cast<long long>(cta) * p.kv_heads + kvh) * 2 + which) * kRows;
+}
+
+template <int NG, bool kBf16>
+__global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(const KvAttnParams p) {
+  constexpr int D = 32 * NG, Q = NG < 4 ? NG : 4, NQ = NG / Q;
   constexpr int kBytes = kv_block_bytes(D);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(8) unsigned long long bars[kWarps * kSlots];
-  __shared__ long long parts[kWarps];
-  __shared__ int found[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int item = blockIdx.x, kvh = blockIdx.y;
+  const int cta = blockIdx.x, kvh = blockIdx.y;
 
-  if (tid < kWarps * kSlots) mbar_init(smem_addr(bars + tid), 1);
+  if (lane < kSlots) mbar_init(smem_addr(bars + warp * kSlots + lane), 2);  // the warp's own
   fence_mbar_init();
-  if (tid == 0) found[0] = -1;
+  __syncwarp();
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // ---- the item: total blocks over all requests give the run length, a second pass finds the request
-  long long mine = 0, before = 0;
-  bool bad = false;
-  for (int i = tid; i < p.requests; i += kThreads) {
-    const Request r = load_request(p, i);
-    bad |= r.bad;
-    if (r.valid) mine += static_cast<long long>((r.fresh * p.group + ROWS - 1) / ROWS) * blocks_of(r.length);
-  }
-  if (bad && item == 0 && kvh == 0) record_status(p.status, kStatusBadLength);
-  const long long all = cta_scan(mine, parts, before);
-  long long want = (all * p.kv_heads + p.target - 1) / p.target;
-  const int run_blocks = static_cast<int>(want > kMinRun ? want : kMinRun);
-  long long carry = 0;
-  for (int base = 0; base < p.requests; base += kThreads) {
-    const int i = base + tid;
-    Request r{};
-    int runs = 0, tiles = 0;
-    if (i < p.requests) {
-      r = load_request(p, i);
-      if (r.valid) {
-        tiles = (r.fresh * p.group + ROWS - 1) / ROWS;
-        runs = (blocks_of(r.length) + run_blocks - 1) / run_blocks;
-      }
-    }
-    const long long n = static_cast<long long>(tiles) * runs;
-    const long long total = cta_scan(n, parts, before);
-    const long long at = item - carry - before;
-    if (at >= 0 && at < n) {
-      found[0] = i;
-      found[1] = static_cast<int>(at) / runs;  // tile
-      found[2] = static_cast<int>(at) % runs;
-      found[3] = runs;
-      found[4] = r.length;
-      found[5] = r.fresh;
-      found[6] = r.token0;
-    }
-    carry += total;
-    if (item < carry) break;  // uniform: every thread sees the same sums
-  }
-  __syncthreads();
-  const int request = found[0];
-  if (request < 0) {
-    if (tid == 0 && kvh == 0) p.headers[item].runs = 0;
-    return;
-  }
-  const int tile = found[1], run = found[2], runs = found[3], length = found[4], fresh = found[5], token0 = found[6];
-  const int row0 = tile * ROWS, rows = min(ROWS, fresh * p.group - row0);
+  Share it = find_share(p, cta, gridDim.x, cta == 0 && kvh == 0 && warp == 0);
   if (tid == 0 && kvh == 0) {
-    RunHeader h{};
-    h.run = run, h.runs = runs, h.rows = rows, h.row0 = row0, h.token0 = token0;
-    p.headers[item] = h;
+    Header h{};
+    h.last = -1;
+    if (it.pos < it.end && it.unit > 0) {  // the share begins inside a segment: others hold its beginning
+      const int begin = it.pos - it.unit;
+      h.first = begin / it.share;
+      h.last = (begin + it.r.units - 1) / it.share;
+      h.row0 = it.tile * kRows;
+      h.rows = min(kRows, it.r.fresh * p.group - h.row0);
+      h.token0 = it.r.token0;
+    }
+    p.headers[cta] = h;
   }
-  const int first_block = run * run_blocks;
-  const int last_block = min(first_block + run_blocks, length > 0 ? blocks_of(length) : 0);
-  const int count = max(0, (last_block - first_block - warp + kWarps - 1) / kWarps);  // this warp's blocks
-  const int* table = p.table + static_cast<long long>(request) * p.width;
-  const int per_page_shift = p.page_shift - 4;
-
-  // ---- the warp's ring: block s of the warp is block first_block + warp + s * kWarps of the request
-  const unsigned ring = smem_addr(smem) + warp * kSlots * kBytes;
+  const unsigned ring = smem_addr(smem) + warp * kSlots * 2 * kBytes;
   const unsigned bar0 = smem_addr(bars + warp * kSlots);
-  unsigned skipped = 0;  // slots whose page is no page: nothing is copied and the block counts as masked
-  int entry = -1;        // table entries of 32 blocks, one per lane
-  auto issue = [&](int s) {
-    if ((s & 31) == 0) {
-      const int block = first_block + warp + (s + lane) * kWarps;
-      entry = s + lane < count ? __ldg(table + (block >> per_page_shift)) : -1;
-    }
-    const int id = __shfl_sync(0xffffffffu, entry, s & 31), slot = s % kSlots;
-    if (id < 0 || id >= p.num_pages) {
-      skipped |= 1u << slot;
-      if (lane == 0) record_status(p.status, kStatusBadPage);
-      return;
-    }
-    skipped &= ~(1u << slot);
-    if (lane == 0) {
-      const int block = first_block + warp + s * kWarps;
-      const long long at =
-          ((static_cast<long long>(id) * p.kv_heads + kvh) << per_page_shift) + (block & ((1 << per_page_shift) - 1));
-      fence_proxy_async_smem();  // the slot's last block was read by ordinary loads
-      mbar_arrive_expect_tx(bar0 + 8 * slot, kBytes);
-      bulk_g2s(ring + slot * kBytes, p.pages + at * kBytes, kBytes, bar0 + 8 * slot);
-    }
-  };
-  for (int s = 0; s < kSlots && s < count; ++s) issue(s);
+  float* wo = reinterpret_cast<float*>(smem + kWarps * kSlots * 2 * kBytes);  // [warp][row][dim]
+  float2* ws = reinterpret_cast<float2*>(wo + kWarps * kRows * D);             // [warp][row] (ref, sum)
+  const int per_page_shift = p.page_shift - 4;
+  int turn = 0;  // units this warp has sent through its ring before this piece
 
-  // ---- q as B fragments: row g of each 8-row tile, times a power of two; -8 * 2^-24 * sum q per group
-  unsigned qb[NT][NG][4];
-  float c0[NT][NG][2];        // accumulator start of rows 2 t, 2 t + 1
-  float rs[NT][2];            // score factor of rows 2 t, 2 t + 1: scale * log2(e) * 2^24 / (q's power of two)
-  int limit[NT][2];           // positions that rows 2 t, 2 t + 1 see
-  int least = INT_MAX;        // the smallest limit of the tile
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = nt * 8 + g;
-    const bool there = row < rows;
-    const int at = row0 + row, token = at / p.group;
+  while (it.pos < it.end) {
+    // ---- one piece: units [it.unit, last_unit) of a segment
+    const int last_unit = min(it.r.units, it.unit + it.end - it.pos);
+    const int length = it.r.length, fresh = it.r.fresh, token0 = it.r.token0;
+    const int row0 = it.tile * kRows, rows = min(kRows, fresh * p.group - row0);
+    // q's rows, asked for before the table is waited for: row g of each 8-row tile, dims 32 G + 8 t .. + 7.
+    uint4 qw[NG];
+    const int row = g, at = row0 + row, token = by_group(p, at);
     const unsigned short* src = p.q + (token0 + token) * p.q_stride +
                                 static_cast<long long>(kvh * p.group + at - token * p.group) * D;
-    uint4 w[NG];
 #pragma unroll
     for (int G = 0; G < NG; ++G)
-      w[G] = there ? __ldg(reinterpret_cast<const uint4*>(src + 32 * G + 8 * t)) : make_uint4(0u, 0u, 0u, 0u);
+      qw[G] = row < rows ? __ldg(reinterpret_cast<const uint4*>(src + 32 * G + 8 * t)) : make_uint4(0u, 0u, 0u, 0u);
+    // Units of two blocks (32 tokens) go to the warps in turn; unit s of this warp begins at block first_block + 2 * (warp +
+    // 4 * s).
+    const int first_block = 2 * it.unit, last_block = (length + kKvBlock - 1) / kKvBlock;
+    const int units = p.whole ? (length + kUnitTokens - 1) / kUnitTokens : last_unit - it.unit;
+    const int count = max(0, (units - warp + kWarps - 1) / kWarps);
+    const int* table = p.table + static_cast<long long>(it.request) * p.width;
+
+    // ---- the warp's ring. Lane 2 u + b keeps the address of block b of unit u of a window of 16 units and issues its copy;
+    // a page that is no page (or a block behind the last) is not copied, its tokens are masked.
+    const unsigned char* source = nullptr;
+    unsigned issued_ok = 0;  // blocks of the window being issued that have a page
+    auto issue = [&](int s) {
+      const int u = s & 15, slot = (turn + s) % kSlots;
+      if (u == 0) {
+        const int block = first_block + 2 * (warp + kWarps * (s + (lane >> 1))) + (lane & 1);
+        const bool there = block < last_block;
+        const int id = there ? __ldg(table + (block >> per_page_shift)) : -1;
+        const bool page = id >= 0 && id < p.num_pages;
+        if (there && !page) record_status(p.status, kStatusBadPage);
+        const long long at =
+            ((static_cast<long long>(id) * p.kv_heads + kvh) << per_page_shift) + (block & ((1 << per_page_shift) - 1));
+        source = page ? p.pages + at * kBytes : nullptr;
+        issued_ok = __ballot_sync(0xffffffffu, page);
+      }
+      if ((lane >> 1) == u) {
+        if (turn + s >= kSlots) fence_proxy_async_smem();  // the slot's last blocks were read by ordinary loads
+        mbar_arrive_expect_tx(bar0 + 8 * slot, source ? kBytes : 0);
+        if (source) bulk_g2s(ring + (slot * 2 + (lane & 1)) * kBytes, source, kBytes, bar0 + 8 * slot);
+      }
+    };
+    for (int s = 0; s < kSlots && s < count; ++s) issue(s);
+
+    // ---- q as B fragments, times a power of two of its row
+    unsigned qb[NG][4];
+    unsigned offset[2];     // B fragment of -8 * 2^-24 * sum q, see below
+    float rs[2];            // score factor of rows 2 t, 2 t + 1: scale * log2(e) * 2^24 / (q's power of two)
+    int limit[2];           // positions that rows 2 t, 2 t + 1 see
     float top = 0.0f;
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
-      const unsigned u[4] = {w[G].x, w[G].y, w[G].z, w[G].w};
+      const unsigned u[4] = {qw[G].x, qw[G].y, qw[G].z, qw[G].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         top = fmaxf(top, fmaxf(fabsf(kBf16 ? bf16lo(u[e]) : f16lo(u[e])), fabsf(kBf16 ? bf16hi(u[e]) : f16hi(u[e]))));
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int ef = max(static_cast<int>(__float_as_uint(top) >> 23), 11);
-    const float up = __uint_as_float(static_cast<unsigned>(264 - ef) << 23);  // 2^(137 - ef): the maximum becomes < 2^11
-    const float mine_rs = p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 10) << 23) * 16777216.0f;
-    float group_sum[NG];
+    const int ef = max(static_cast<int>(__float_as_uint(top) >> 23), 15);
+    const float up = __uint_as_float(static_cast<unsigned>(268 - ef) << 23);  // 2^(141 - ef): the maximum becomes < 2^15
+    const float mine_rs = p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 14) << 23) * 16777216.0f;
+    float c0[NG][2];  // of rows 2 t, 2 t + 1
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
-      const unsigned u[4] = {w[G].x, w[G].y, w[G].z, w[G].w};
+      const unsigned u[4] = {qw[G].x, qw[G].y, qw[G].z, qw[G].w};
       float x[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -320,330 +380,420 @@ __global__ void __launch_bounds__(kThreads) kv_attn_kernel(const KvAttnParams p)
         x[2 * e + 1] = (kBf16 ? bf16hi(u[e]) : f16hi(u[e])) * up;
       }
       // nibble pairs (0, 4), (1, 5) * 16, (2, 6), (3, 7) * 16
-      float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float by = e & 1 ? 0.0625f : 1.0f;
-        const unsigned pair = pack_h2(x[e] * by, x[e + 4] * by);
-        qb[nt][G][e] = pair;
-        sum += (f16lo(pair) + f16hi(pair)) * (e & 1 ? 16.0f : 1.0f);
+        qb[G][e] = pack_h2(x[e] * by, x[e + 4] * by);
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      group_sum[G] = sum * (-8.0f / 16777216.0f);
+      // -2^-21 for the pairs as they are, 16 times that for those that were divided by 16
+      constexpr unsigned kOne = 0x80088008u, kSixteen = 0x80808080u;
+      const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float sum[4];
+      mma_f16(sum, kOne, kOne, kSixteen, kSixteen, qb[G][0], qb[G][1], zero);
+      mma_f16(sum, kOne, kOne, kSixteen, kSixteen, qb[G][2], qb[G][3], sum);
+      c0[G][0] = sum[0], c0[G][1] = sum[1];
+    }
+    // The offsets as a B fragment (k x rows) for an A of the tokens' K scales, in two FP16 terms (2^-25 at worst): slots
+    // k = 2 t, 2 t + 1 (and + 8) of lane (g, t) take a pair of groups' high or low term of row g.
+#pragma unroll
+    for (int half = 0; half < 2; ++half) offset[half] = 0u;
+#pragma unroll
+    for (int i = 0; i < NG / 2; ++i) {
+      float mine[2];  // groups 2 i, 2 i + 1 of row g: lane g / 2 holds rows g & ~1, (g & ~1) + 1
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float even = __shfl_sync(0xffffffffu, c0[2 * i + h][0], g >> 1);
+        const float odd = __shfl_sync(0xffffffffu, c0[2 * i + h][1], g >> 1);
+        mine[h] = g & 1 ? odd : even;
+      }
+      const unsigned high = pack_h2(mine[0], mine[1]);
+      const unsigned low = pack_h2(mine[0] - lo_f32(high), mine[1] - hi_f32(high));
+      if (NG == 8) {
+        if (t == i) offset[0] = high, offset[1] = low;
+      } else {
+        if (t == i) offset[0] = high;
+        if (t == i + NG / 2) offset[0] = low;
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {  // from the lane that holds row 2 t + e as its row g
-      const int from = (2 * t + e) * 4;
-#pragma unroll
-      for (int G = 0; G < NG; ++G) c0[nt][G][e] = __shfl_sync(0xffffffffu, group_sum[G], from);
-      rs[nt][e] = __shfl_sync(0xffffffffu, mine_rs, from);
-      const int r = nt * 8 + 2 * t + e;
-      limit[nt][e] = r < rows ? length - fresh + (row0 + r) / p.group + 1 : 0;
+    for (int e = 0; e < 2; ++e) {  // from a lane that holds row 2 t + e as its row g
+      rs[e] = __shfl_sync(0xffffffffu, mine_rs, (2 * t + e) * 4);
+      const int r = 2 * t + e;
+      limit[e] = r < rows ? length - fresh + by_group(p, row0 + r) + 1 : 0;
     }
-  }
-  least = length - fresh + row0 / p.group + 1;
-  if (rows < ROWS) least = min(least, length);  // rows that are not there: masked or not, they are never written
+    // The smallest limit of the tile; rows that are not there are never written, masked or not.
+    const int least = length - fresh + by_group(p, row0) + 1;
 
-  float o[NT][2 * NG][4], ones[NT][NG][4], l[NT][2], ref[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+    // ones = sum of P' per group; groups 2 i and 2 i + 1 share an accumulator (rows 0-7 and 8-15 of the A operand).
+    float o[2 * NG][4], ones[NG / 2][4], l[2], nref[2];  // nref = -ref
 #pragma unroll
     for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
 #pragma unroll
-    for (int G = 0; G < NG; ++G)
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) ones[nt][G][e] = 0.0f;
-    l[nt][0] = l[nt][1] = 0.0f;
-    ref[nt][0] = ref[nt][1] = kNegInf;
-  }
-  int vexp = -3;                    // log2 of the V scales that `ref` allows for (below 2^3 of it)
-  unsigned vbound = 0u;             // 2^(vexp + 3) as an FP16 pair; 0 until the first block
-  unsigned phases = 0;              // parity of each slot
-  bool live = true;
+      for (int i = 0; i < NG / 2; ++i) ones[i][e] = 0.0f;
+    l[0] = l[1] = 0.0f;
+    nref[0] = nref[1] = -kNegInf;
+    const int tv = kBf16 ? t : g >> 1;  // the token pair whose V scales this lane holds
+    int vshift = 0;                     // V scales are taken times 2^-vshift, which is below 2
+    unsigned ok = 0;            // blocks of the window being read that have a page
+    bool live = true;
 
-  for (int s = 0; s < count; ++s) {
-    const int slot = s % kSlots, block = first_block + warp + s * kWarps;
-    if (skipped >> slot & 1) {
-      if (s + kSlots < count) issue(s + kSlots);
-      continue;
-    }
-    if (!mbar_wait(bar0 + 8 * slot, phases >> slot & 1)) {
-      if (lane == 0) record_status(p.status, kStatusMbarTimeout);
-      live = false;
-    }
-    live = __all_sync(0xffffffffu, live);
-    if (!live) {  // leave, after a bounded wait for the warp's other copies in flight
-      for (int k = s + 1; k < count && k < s + kSlots; ++k)
-        if (!(skipped >> (k % kSlots) & 1)) (void)mbar_wait(bar0 + 8 * (k % kSlots), phases >> (k % kSlots) & 1);
-      break;
-    }
-    phases ^= 1u << slot;
-    const unsigned at = ring + slot * kBytes;
-    // K words of tokens g, g + 8; V words of tokens 2 t, 2 t + 1 (j = 0) and 2 t + 8, 2 t + 9 (j = 1)
-    unsigned kw[2][NG], vw[2][NG], sv[2][NG], kscale[2][NG / 2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int quad = 0; quad < NQ; ++quad) {
-        unsigned a[Q];
-        lds_words<Q>(at + quad * (256 * Q) + (g + 8 * j) * (16 * Q) + t * (4 * Q), a);
-#pragma unroll
-        for (int i = 0; i < Q; ++i) kw[j][quad * Q + i] = a[i];
-        lds_words<Q>(at + 8 * D + quad * (256 * Q) + j * (128 * Q) + g * (16 * Q) + t * (4 * Q), a);
-#pragma unroll
-        for (int i = 0; i < Q; ++i) vw[j][quad * Q + i] = a[i];
+    for (int s = 0; s < count; ++s) {
+      const int slot = (turn + s) % kSlots;
+      if ((s & 15) == 0) ok = issued_ok;
+      const int pos = (first_block + 2 * (warp + kWarps * s)) * kKvBlock;
+      live = mbar_wait(bar0 + 8 * slot, (turn + s) / kSlots & 1);
+      live = __all_sync(0xffffffffu, live);
+      if (!live) {  // leave, after a bounded wait for the warp's other copies in flight
+        if (lane == 0) record_status(p.status, kStatusMbarTimeout);
+        for (int k = s + 1; k < count && k < s + kSlots; ++k) 
+          (void)mbar_wait(bar0 + 8 * ((turn + k) % kSlots), (turn + k) / kSlots & 1);
+        break;
       }
-      lds_words<NG / 2>(at + 16 * D + (g + 8 * j) * (2 * NG), kscale[j]);
-      lds_words<NG>(at + 17 * D + (j * 4 + t) * (4 * NG), sv[j]);
-    }
-    __syncwarp();
-    if (s + kSlots < count) issue(s + kSlots);
+      const unsigned at = ring + slot * 2 * kBytes;
 
-    const int pos = block * kKvBlock;
-    if (pos + kKvBlock > length) {  // tokens that are not there: scales whatever they are become 0
+      // ---- S^T = K Q^T of tokens g, g + 8 of both blocks
+      float x[2][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int token = pos + 8 * j + 2 * t;
-        const unsigned keep = (token < length ? 0x0000ffffu : 0u) | (token + 1 < length ? 0xffff0000u : 0u);
+      for (int b = 0; b < 2; ++b) {
+        unsigned kw[2][NG], kscale[2][NG / 2], kpair[2];
 #pragma unroll
-        for (int G = 0; G < NG; ++G) sv[j][G] &= keep;
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int quad = 0; quad < NQ; ++quad) {
+            unsigned a[Q];
+            lds_words<Q>(at + b * kBytes + quad * (256 * Q) + (g + 8 * j) * (16 * Q) + t * (4 * Q), a);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) kw[j][quad * Q + i] = a[i];
+          }
+          lds_words<NG / 2>(at + b * kBytes + 16 * D + (g + 8 * j) * (2 * NG), kscale[j]);
+          kpair[j] = lds32(at + b * kBytes + 16 * D + (g + 8 * j) * (2 * NG) + 4 * (t & (NG / 2 - 1)));
+        }
+        const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_f16(x[b], kpair[0], kpair[1], NG == 8 ? kpair[0] : 0u, NG == 8 ? kpair[1] : 0u, offset[0],
+                offset[1], zero);
+#pragma unroll
+        for (int G = 0; G < NG; ++G) {
+          const unsigned a = kw[0][G], c = kw[1][G], ah = a >> 8, ch = c >> 8;
+          const float s0 = G & 1 ? hi_f32(kscale[0][G / 2]) : lo_f32(kscale[0][G / 2]);
+          const float s1 = G & 1 ? hi_f32(kscale[1][G / 2]) : lo_f32(kscale[1][G / 2]);
+          float acc[4];
+          const float start[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16(acc, a & 0x000f000fu, c & 0x000f000fu, a & 0x00f000f0u, c & 0x00f000f0u, qb[G][0], qb[G][1],
+                  start);
+          mma_f16(acc, ah & 0x000f000fu, ch & 0x000f000fu, ah & 0x00f000f0u, ch & 0x00f000f0u, qb[G][2],
+                  qb[G][3], acc);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float by = e & 2 ? s1 : s0;
+            x[b][e] = fmaf(acc[e], by, x[b][e]);
+          }
+        }
       }
-    }
 
-    // ---- S^T = K Q^T
-    float x[NT][4];
+      // ---- V scales of tokens 2 tv, 2 tv + 1 (j = 0) and 2 tv + 8, 2 tv + 9 (j = 1), and scores against the reference
+      unsigned sv[2][2][NG];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[nt][e] = 0.0f;
+        for (int j = 0; j < 2; ++j)
+          lds_words<NG>(at + b * kBytes + 17 * D + (j * 4 + tv) * (4 * NG), sv[b][j]);
+      float y[2][4];
 #pragma unroll
-    for (int G = 0; G < NG; ++G) {
-      const unsigned a = kw[0][G], b = kw[1][G], ah = a >> 8, bh = b >> 8;
-      const float s0 = G & 1 ? f16hi(kscale[0][G / 2]) : f16lo(kscale[0][G / 2]);
-      const float s1 = G & 1 ? f16hi(kscale[1][G / 2]) : f16lo(kscale[1][G / 2]);
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float acc[4];
-        const float start[4] = {c0[nt][G][0], c0[nt][G][1], c0[nt][G][0], c0[nt][G][1]};
-        mma_f16(acc, a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u, qb[nt][G][0], qb[nt][G][1],
-                start);
-        mma_f16(acc, ah & 0x000f000fu, bh & 0x000f000fu, ah & 0x00f000f0u, bh & 0x00f000f0u, qb[nt][G][2],
-                qb[nt][G][3], acc);
-        x[nt][0] = fmaf(acc[0], s0, x[nt][0]);
-        x[nt][1] = fmaf(acc[1], s0, x[nt][1]);
-        x[nt][2] = fmaf(acc[2], s1, x[nt][2]);
-        x[nt][3] = fmaf(acc[3], s1, x[nt][3]);
+        for (int e = 0; e < 4; ++e) y[b][e] = fmaf(x[b][e], rs[e & 1], nref[e & 1]);
+      if (pos + 2 * kKvBlock > least || (ok >> 2 * (s & 15) & 3u) != 3u) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const bool page = ok >> (2 * (s & 15) + b) & 1;
+          const int end = page ? length : 0, first = pos + b * kKvBlock;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {  // tokens that are not there: scales whatever they are become 0
+            const int token = first + 8 * j + 2 * tv;
+            const unsigned keep = (token < end ? 0x0000ffffu : 0u) | (token + 1 < end ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int G = 0; G < NG; ++G) sv[b][j][G] &= keep;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (first + g + (e & 2 ? 8 : 0) >= min(end, limit[e & 1])) x[b][e] = y[b][e] = kNegInf;
+        }
       }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[nt][e] *= rs[nt][e & 1];
-    if (pos + kKvBlock > least) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (pos + g + (e & 2 ? 8 : 0) >= limit[nt][e & 1]) x[nt][e] = kNegInf;
-    }
 
-    // ---- does the reference still hold? P' = 2^(x - ref) * V scale stays below 2^15
-    unsigned vtop = max_h2(sv[0][0], sv[1][0]);
+      // ---- does the reference still hold, and are the V scales below 2 (bit 14 of a positive FP16 says so)?
+      if (vshift) {
+        const unsigned by = static_cast<unsigned>((15 - vshift) << 10) * 0x10001u;  // 2^-vshift, vshift <= 15
 #pragma unroll
-    for (int G = 1; G < NG; ++G) vtop = max_h2(vtop, max_h2(sv[0][G], sv[1][G]));
-    bool move = max_h2(vtop, vbound) != vbound;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) move |= x[nt][e] > ref[nt][e & 1] + (8.0f + kSlack) - static_cast<float>(vexp);
-    if (__any_sync(0xffffffffu, move)) {
+            for (int G = 0; G < NG; ++G) sv[b][j][G] = mul_h2(sv[b][j][G], by);
+      }
+      unsigned any = 0u;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) vtop = max_h2(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-      const float v = fmaxf(f16lo(vtop), f16hi(vtop));
-      const int exponent = static_cast<int>(__float_as_uint(v) >> 23) - 126;  // v < 2^exponent
-      const int old = vexp;
-      vexp = max(vexp, exponent);
-      // 2^(vexp + 3) where FP16 has it, its largest finite value above that
-      const int bits = vexp + 3 < 16 ? (vexp + 18) << 10 : 0x7bff;
-      vbound = static_cast<unsigned>(bits) * 0x10001u;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int G = 0; G < NG; ++G) any |= sv[b][0][G] | sv[b][1][G];
+      float most = kNegInf;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) most = fmaxf(most, fmaxf(y[b][e], y[b][e + 1]));
+      if (__any_sync(0xffffffffu, most > kMoveAt || (any & 0x40004000u))) {
+        unsigned vtop = 0u;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int G = 0; G < NG; ++G) vtop = max_h2(vtop, max_h2(sv[b][0][G], sv[b][1][G]));
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) vtop = max_h2(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
+        // v < 2^exponent; the scales become those below 2
+        const float v = fmaxf(lo_f32(vtop), hi_f32(vtop));
+        const int more = max(0, static_cast<int>(__float_as_uint(v) >> 23) - 126 - 1);
+        const float by_shift = __int_as_float((127 - more) << 23);
+        if (more) {
+          const unsigned by = static_cast<unsigned>((15 - more) << 10) * 0x10001u;
+          vshift += more;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int G = 0; G < NG; ++G) sv[b][j][G] = mul_h2(sv[b][j][G], by);
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(x[nt][e], x[nt][e + 2]);
+          float top = fmaxf(fmaxf(x[0][e], x[0][e + 2]), fmaxf(x[1][e], x[1][e + 2])) * rs[e];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          // ref = (largest score so far) - 8 + vexp
-          const float was = ref[nt][e];
-          const float now = fmaxf(top - 8.0f, was - static_cast<float>(old)) + static_cast<float>(vexp);
-          const float factor = was == kNegInf ? 0.0f : exp2_fast(was - now);
+          const float was = -nref[e], now = fmaxf(top - kRefBelow, was);
           if (was != kNegInf) {
-            l[nt][e] *= factor;
+            float factor = exp2_fast(was - now);
+            l[e] *= factor;
+            factor *= by_shift;
 #pragma unroll
-            for (int i = 0; i < 2 * NG; ++i) o[nt][i][e] *= factor, o[nt][i][e + 2] *= factor;
+            for (int i = 0; i < 2 * NG; ++i) o[i][e] *= factor, o[i][e + 2] *= factor;
 #pragma unroll
-            for (int G = 0; G < NG; ++G) ones[nt][G][e] *= factor, ones[nt][G][e + 2] *= factor;
+            for (int i = 0; i < NG / 2; ++i) ones[i][e] *= factor, ones[i][e + 2] *= factor;
           }
-          ref[nt][e] = now;
+          nref[e] = -now;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int h = 0; h < 4; h += 2) {
+              const float v = x[b][e + h];
+              y[b][e + h] = v == kNegInf ? kNegInf : fmaf(v, rs[e], -now);
+            }
         }
-    }
-
-    // ---- P, its sums, and P' per group as B fragments (rows x tokens)
-    unsigned pb[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float r = ref[nt][e & 1];
-        w[e] = exp2_fast(x[nt][e] - (r == kNegInf ? 0.0f : r));
       }
-      l[nt][0] += w[0] + w[2];
-      l[nt][1] += w[1] + w[3];
-      pb[nt][0] = transpose8x8(pack_h2(w[0], w[1]));
-      pb[nt][1] = transpose8x8(pack_h2(w[2], w[3]));
-    }
 
-    // ---- O^T += V^T P'
+      // ---- P, its sums, P' per group as B fragments (rows x tokens), O^T += V^T P'
 #pragma unroll
-    for (int G = 0; G < NG; ++G) {
-      const unsigned a = vw[0][G], b = vw[1][G], ah = a >> 8, bh = b >> 8;
+      for (int b = 0; b < 2; ++b) {
+        unsigned pb[2], vw[2][NG];
+        float w[4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const unsigned b0 = mul_h2(pb[nt][0], sv[0][G]), b1 = mul_h2(pb[nt][1], sv[1][G]);
-        mma_f16(o[nt][2 * G], a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u, b0, b1,
-                o[nt][2 * G]);
-        mma_f16(o[nt][2 * G + 1], ah & 0x000f000fu, ah & 0x00f000f0u, bh & 0x000f000fu, bh & 0x00f000f0u, b0, b1,
-                o[nt][2 * G + 1]);
-        mma_f16(ones[nt][G], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b0, b1, ones[nt][G]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int quad = 0; quad < NQ; ++quad) {
+            unsigned a[Q];
+            lds_words<Q>(at + b * kBytes + 8 * D + quad * (256 * Q) + j * (128 * Q) + g * (16 * Q) + t * (4 * Q), a);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) vw[j][quad * Q + i] = a[i];
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = exp2_fast(y[b][e]);
+        l[0] += w[0] + w[2];
+        l[1] += w[1] + w[3];
+        if (kBf16) {
+          pb[0] = transpose8x8(pack_h2(w[0], w[1]));
+          pb[1] = transpose8x8(pack_h2(w[2], w[3]));
+        }
+#pragma unroll
+        for (int G = 0; G < NG; ++G) {
+          const unsigned a = vw[0][G], c = vw[1][G], ah = a >> 8, ch = c >> 8;
+          float s0 = 0.0f, s1 = 0.0f;
+          if (!kBf16) {
+            s0 = f16_to_f32(static_cast<unsigned short>(sv[b][0][G] >> (16 * (g & 1))));
+            s1 = f16_to_f32(static_cast<unsigned short>(sv[b][1][G] >> (16 * (g & 1))));
+          }
+          unsigned b0, b1;
+          if (kBf16) {
+            b0 = mul_h2(pb[0], sv[b][0][G]), b1 = mul_h2(pb[1], sv[b][1][G]);
+          } else {
+            b0 = transpose8x8(pack_h2(w[0] * s0, w[1] * s0));
+            b1 = transpose8x8(pack_h2(w[2] * s1, w[3] * s1));
+          }
+          mma_f16(o[2 * G], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, b0, b1,
+                  o[2 * G]);
+          mma_f16(o[2 * G + 1], ah & 0x000f000fu, ah & 0x00f000f0u, ch & 0x000f000fu, ch & 0x00f000f0u, b0, b1,
+                  o[2 * G + 1]);
+          constexpr unsigned kOnes = 0x3c003c00u;
+          if (G & 1)
+            mma_f16(ones[G / 2], 0u, kOnes, 0u, kOnes, b0, b1, ones[G / 2]);
+          else
+            mma_f16(ones[G / 2], kOnes, 0u, kOnes, 0u, b0, b1, ones[G / 2]);
+        }
       }
+      __syncwarp();
+      if (s + kSlots < count) issue(s + kSlots);
     }
-  }
 
-  // ---- the warps' sums over the ring's memory: [warp][row][dim] and (ref, sum) per warp and row
-  __syncthreads();
-  float* wo = reinterpret_cast<float*>(smem);
-  float2* ws = reinterpret_cast<float2*>(smem + static_cast<size_t>(kWarps) * ROWS * D * 4);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    turn += count;
+
+    // ---- the warps' sums to shared memory, joined there
+    const float unshift = __int_as_float((127 + vshift) << 23);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float sum = l[nt][e];
+      float sum = l[e];
 #pragma unroll
       for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const int row = nt * 8 + 2 * t + e;
-      if (g == 0) ws[warp * ROWS + row] = make_float2(ref[nt][e], sum);
-      float* to = wo + (warp * ROWS + row) * D;
+      const int row = 2 * t + e;
+      if (g == 0) ws[warp * kRows + row] = make_float2(-nref[e], sum);
+      float* to = wo + (warp * kRows + row) * D;
 #pragma unroll
       for (int G = 0; G < NG; ++G) {
-        const float eight = 8.0f * ones[nt][G][e];
+        const float mass = ones[G / 2][G & 1 ? e + 2 : e];
+        const float eight = 8.0f * unshift * mass;
         float4 v;
-        v.x = fmaf(o[nt][2 * G][e], 16777216.0f, -eight);
-        v.y = fmaf(o[nt][2 * G][e + 2], 1048576.0f, -eight);
-        v.z = fmaf(o[nt][2 * G + 1][e], 16777216.0f, -eight);
-        v.w = fmaf(o[nt][2 * G + 1][e + 2], 1048576.0f, -eight);
+        v.x = fmaf(o[2 * G][e], 16777216.0f * unshift, -eight);
+        v.y = fmaf(o[2 * G][e + 2], 1048576.0f * unshift, -eight);
+        v.z = fmaf(o[2 * G + 1][e], 16777216.0f * unshift, -eight);
+        v.w = fmaf(o[2 * G + 1][e + 2], 1048576.0f * unshift, -eight);
         *reinterpret_cast<float4*>(to + 32 * G + 4 * g) = v;
       }
     }
-  __syncthreads();
-  constexpr int kVec = D / 4;  // float4s of a row
-  for (int at = tid; at < rows * kVec; at += kThreads) {
-    const int row = at / kVec, c = at - row * kVec;
-    float top = kNegInf;
+    __syncthreads();
+    constexpr int kVec = D / 4;  // float4s of a row
+    for (int at = tid; at < rows * kVec; at += kThreads) {
+      const int row = at / kVec, c = at - row * kVec;
+      float top = kNegInf;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ws[w * ROWS + row].x);
-    float den = 0.0f;
-    float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ws[w * kRows + row].x);
+      float den = 0.0f;
+      float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float2 st = ws[w * ROWS + row];
-      if (st.x == kNegInf && st.y == 0.0f) continue;  // a warp that saw nothing of this row
-      const float f = exp2_fast(st.x - top);
-      const float4 v = *reinterpret_cast<const float4*>(wo + (w * ROWS + row) * D + 4 * c);
-      den = fmaf(f, st.y, den);
-      num.x = fmaf(f, v.x, num.x), num.y = fmaf(f, v.y, num.y), num.z = fmaf(f, v.z, num.z), num.w = fmaf(f, v.w, num.w);
-    }
-    if (runs == 1) {
-      const float by = den == 0.0f ? 0.0f : __frcp_rn(den);  // a row that sees no position: 0
-      const int r = row0 + row, token = r / p.group;
-      unsigned short* to = p.out + (static_cast<long long>(token0 + token) * p.heads + kvh * p.group + r - token * p.group) * D;
-      uint2 w;
-      if (kBf16) {
-        w.x = f32_to_bf16_rn(num.x * by) | static_cast<unsigned>(f32_to_bf16_rn(num.y * by)) << 16;
-        w.y = f32_to_bf16_rn(num.z * by) | static_cast<unsigned>(f32_to_bf16_rn(num.w * by)) << 16;
-      } else {
-        w.x = pack_h2(num.x * by, num.y * by);
-        w.y = pack_h2(num.z * by, num.w * by);
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 st = ws[w * kRows + row];
+        if (st.x == kNegInf && st.y == 0.0f) continue;  // a warp that saw nothing of this row
+        const float f = exp2_fast(st.x - top);
+        const float4 v = *reinterpret_cast<const float4*>(wo + (w * kRows + row) * D + 4 * c);
+        den = fmaf(f, st.y, den);
+        num.x = fmaf(f, v.x, num.x), num.y = fmaf(f, v.y, num.y), num.z = fmaf(f, v.z, num.z), num.w = fmaf(f, v.w, num.w);
       }
-      reinterpret_cast<uint2*>(to)[c] = w;
-    } else {
-      const long long rec = (static_cast<long long>(item) * p.kv_heads + kvh) * ROWS + row;
-      if (c == 0) p.stats[rec] = make_float2(top, den);
-      reinterpret_cast<float4*>(p.sums + rec * D)[c] = num;
+      if (it.unit == 0 && last_unit == it.r.units) {
+        const float by = den == 0.0f ? 0.0f : __frcp_rn(den);  // a row that sees no position: 0
+        const int r = row0 + row, token = by_group(p, r);
+        unsigned short* to = p.out + (static_cast<long long>(token0 + token) * p.heads + kvh * p.group + r - token * p.group) * D;
+        uint2 w;
+        if (kBf16) {
+          w.x = f32_to_bf16_rn(num.x * by) | static_cast<unsigned>(f32_to_bf16_rn(num.y * by)) << 16;
+          w.y = f32_to_bf16_rn(num.z * by) | static_cast<unsigned>(f32_to_bf16_rn(num.w * by)) << 16;
+        } else {
+          w.x = pack_h2(num.x * by, num.y * by);
+          w.y = pack_h2(num.z * by, num.w * by);
+        }
+        reinterpret_cast<uint2*>(to)[c] = w;
+      } else {  // record 0: a piece that continues a segment, record 1: one that begins it
+        const long long rec = record_of(p, cta, kvh, it.unit == 0) + row;
+        if (c == 0) p.stats[rec] = make_float2(top, den);
+        reinterpret_cast<float4*>(p.sums + rec * D)[c] = num;
+      }
     }
+    it.pos += last_unit - it.unit;
+    if (!__syncthreads_and(live)) return;  // a copy never came: the status says so, nothing more is asked for
+    if (it.pos < it.end) next_segment(p, it);
   }
 }
 
-// Joins the runs of one (request, tile, kv head): the tile's rows are dealt to the CTAs that made the runs. 128 threads =
-// D / 4 float4 columns x the classes that share the runs; the classes' sums are added in order.
-template <int D, int ROWS, bool kBf16>
+// Joins what the CTAs first .. last left of one segment (tile of a request, kv head): record 1 of the first, record 0 of the
+// others. Its rows * D / 4 columns of 4 are dealt to the CTAs behind the first, `each` (a power of two) to a CTA, whose
+// threads share the records of a column in 128 / each classes: every thread reads its records in one go against a reference
+// of its own; classes meet by butterflies inside a warp and in order through shared memory.
+template <int D, bool kBf16>
 __global__ void __launch_bounds__(kThreads) kv_combine_kernel(const KvAttnParams p) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  float4* part = reinterpret_cast<float4*>(smem);             // [classes][columns]
-  float* weight = reinterpret_cast<float*>(smem + 16 * kThreads);  // [runs]
-  __shared__ float red[2 * kWarps];
+  __shared__ float4 part[kThreads];
+  __shared__ float2 part_stat[kThreads];
   grid_dependency_wait();
   grid_launch_dependents();
-  const RunHeader h = p.headers[blockIdx.x];
-  if (h.runs <= 1) return;
+  const Header h = p.headers[blockIdx.x];
+  if (h.last < 0) return;
   const int kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kCols = D / 4, kClasses = kThreads / kCols;
-  const int col = tid % kCols, cls = tid / kCols;
-  const long long first = blockIdx.x - h.run;
-  for (int row = h.run; row < h.rows; row += h.runs) {
-    auto record = [&](int k) { return ((first + k) * p.kv_heads + kvh) * ROWS + row; };
-    float top = kNegInf;
-    for (int k = tid; k < h.runs; k += kThreads) top = fmaxf(top, __ldcg(p.stats + record(k)).x);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[w]);
-    float den = 0.0f;
-    for (int k = tid; k < h.runs; k += kThreads) {
-      const float2 st = __ldcg(p.stats + record(k));
-      const float f = st.x == kNegInf && st.y == 0.0f ? 0.0f : exp2_fast(st.x - top);
-      weight[k] = f;
-      den = fmaf(f, st.y, den);
-    }
-    den = warp_allsum(den);
-    if (lane == 0) red[kWarps + warp] = den;
-    __syncthreads();
-    den = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) den += red[kWarps + w];
+  constexpr int kCols = D / 4;
+  const int parts = h.last - h.first, records = parts + 1, mine = blockIdx.x - h.first - 1;
+  const int total = h.rows * kCols, share = (total + parts - 1) / parts;
+  int shift = 0;
+  while ((1 << shift) < share && shift < 7) ++shift;
+  const int each = 1 << shift, classes = kThreads >> shift, cls = tid >> shift;
+  for (int base = mine * each; base < total; base += parts * each) {
+    const int at = base + (tid & (each - 1)), row = at / kCols, col = at - row * kCols;
+    float top = kNegInf, den = 0.0f;
     float4 num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int k = cls; k < h.runs; k += kClasses) {
-      const float f = weight[k];
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.sums + record(k) * D) + col);
-      if (f != 0.0f)
-        num.x = fmaf(f, v.x, num.x), num.y = fmaf(f, v.y, num.y), num.z = fmaf(f, v.z, num.z), num.w = fmaf(f, v.w, num.w);
-    }
-    part[tid] = num;
-    __syncthreads();
-    if (cls == 0) {
+    for (int k0 = cls; k0 < records; k0 += 4 * classes) {
+      float2 st[4];
+      float4 v[4];
 #pragma unroll
-      for (int k = 1; k < kClasses; ++k) {
-        const float4 v = part[k * kCols + col];
-        num.x += v.x, num.y += v.y, num.z += v.z, num.w += v.w;
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + j * classes;
+        st[j] = make_float2(kNegInf, 0.0f);
+        v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < records && at < total) {
+          const long long record = record_of(p, h.first + k, kvh, k == 0) + row;
+          st[j] = __ldcg(p.stats + record);
+          v[j] = __ldcg(reinterpret_cast<const float4*>(p.sums + record * D) + col);
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) now = fmaxf(now, st[j].x);
+      const float keep = top == kNegInf ? 0.0f : exp2_fast(top - now);
+      if (top != kNegInf) den *= keep, num.x *= keep, num.y *= keep, num.z *= keep, num.w *= keep;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (st[j].x == kNegInf && st[j].y == 0.0f) continue;  // a piece that saw nothing of this row
+        const float f = exp2_fast(st[j].x - now);
+        den = fmaf(f, st[j].y, den);
+        num.x = fmaf(f, v[j].x, num.x), num.y = fmaf(f, v[j].y, num.y);
+        num.z = fmaf(f, v[j].z, num.z), num.w = fmaf(f, v[j].w, num.w);
+      }
+      top = now;
+    }
+    if (each < 32) {  // the classes inside the warp
+      float all = top;
+      for (int d = each; d < 32; d <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, d));
+      if (!(top == kNegInf && den == 0.0f)) {
+        const float f = exp2_fast(top - all);
+        den *= f, num.x *= f, num.y *= f, num.z *= f, num.w *= f;
+      }
+      top = all;
+      for (int d = each; d < 32; d <<= 1) {
+        den += __shfl_xor_sync(0xffffffffu, den, d);
+        num.x += __shfl_xor_sync(0xffffffffu, num.x, d), num.y += __shfl_xor_sync(0xffffffffu, num.y, d);
+        num.z += __shfl_xor_sync(0xffffffffu, num.z, d), num.w += __shfl_xor_sync(0xffffffffu, num.w, d);
+      }
+    }
+    const int step = max(each, 32);  // threads between two classes that are left
+    part[tid] = num;
+    part_stat[tid] = make_float2(top, den);
+    __syncthreads();
+    if (tid < each && at < total) {
+      for (int c = tid + step; c < kThreads; c += step) top = fmaxf(top, part_stat[c].x);
+      den = 0.0f, num = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int c = tid; c < kThreads; c += step) {
+        const float2 st = part_stat[c];
+        if (st.x == kNegInf && st.y == 0.0f) continue;
+        const float f = exp2_fast(st.x - top);
+        const float4 v = part[c];
+        den = fmaf(f, st.y, den);
+        num.x = fmaf(f, v.x, num.x), num.y = fmaf(f, v.y, num.y), num.z = fmaf(f, v.z, num.z), num.w = fmaf(f, v.w, num.w);
       }
       const float by = den == 0.0f ? 0.0f : __frcp_rn(den);
-      const int r = h.row0 + row, token = r / p.group;
+      const int r = h.row0 + row, token = by_group(p, r);
       unsigned short* to = p.out + (static_cast<long long>(h.token0 + token) * p.heads + kvh * p.group + r - token * p.group) * D;
       uint2 w;
       if (kBf16) {
@@ -661,8 +811,8 @@ __global__ void __launch_bounds__(kThreads) kv_combine_kernel(const KvAttnParams
 
 // What a call launches; the grid and the scratch depend on the shapes alone, so a captured call serves any lengths.
 struct KvPlan {
-  int tiles_nt;       // 8-row tiles a CTA holds (1 or 2)
-  int items, target;
+  bool whole;         // segments go to CTAs whole
+  int ctas;           // per kv head
   bool combine;
   size_t headers, stats, sums, total;  // scratch offsets
   size_t smem;
@@ -692,25 +842,24 @@ int kv_plan(int requests, int width, int page_size, int heads, int kv_heads, int
   int sms = 0;
   const int rc = kv_sms(&sms);
   if (rc) return rc;
-  const int most_rows = heads / kv_heads * max_new;
-  plan->tiles_nt = most_rows > 8 && dim < 256 ? 2 : 1;
-  const int rows = 8 * plan->tiles_nt, tiles = (most_rows + rows - 1) / rows;
-  const long long runs = (static_cast<long long>(width) * page_size / kKvBlock + kMinRun - 1) / kMinRun;
-  plan->target = sms * KLAB_KV_CTAS_PER_SM;
-  const long long segments = static_cast<long long>(requests) * tiles;
-  long long items = segments + plan->target / kv_heads + 1;
-  if (segments * runs < items) items = segments * runs;
-  if (items > INT_MAX / 2) return KLAB_E_SHAPE;
-  plan->items = static_cast<int>(items);
-  plan->combine = runs > 1;
+  const int tiles = (heads / kv_heads * max_new + kRows - 1) / kRows;
+  const long long units = (static_cast<long long>(width) * page_size - 1) / kUnitTokens + 1;
+  plan->whole = units <= kWholeUnits;
+  const long long most = static_cast<long long>(requests) * tiles * (plan->whole ? 1 : units);
+  if (most > INT_MAX) return KLAB_E_SHAPE;
+  // One CTA for each place on the machine, dealt evenly to the kv heads; fewer where the table cannot hold more shares.
+  const long long places = static_cast<long long>(sms) * kv_resident(dim / kKvGroup) / kv_heads;
+  const long long shares = plan->whole ? most : (most + kMinShare - 1) / kMinShare;
+  plan->ctas = static_cast<int>(shares < places ? shares : places > 1 ? places : 1);
+  plan->combine = plan->ctas > 1 && !plan->whole;
   plan->headers = 0;
-  plan->stats = (static_cast<size_t>(items) * sizeof(RunHeader) + 127) / 128 * 128;
-  const size_t records = plan->combine ? static_cast<size_t>(items) * kv_heads * rows : 0;
+  plan->stats = (static_cast<size_t>(plan->ctas) * sizeof(Header) + 127) / 128 * 128;
+  const size_t records = plan->combine ? static_cast<size_t>(plan->ctas) * kv_heads * 2 * kRows : 0;
   plan->sums = plan->stats + (records * 8 + 127) / 128 * 128;
   plan->total = plan->sums + records * dim * 4;
-  const size_t ring = static_cast<size_t>(kWarps) * kSlots * kv_block_bytes(dim);
-  const size_t join = static_cast<size_t>(kWarps) * rows * (dim * 4 + 8);
-  plan->smem = ring > join ? ring : join;
+  const size_t ring = static_cast<size_t>(kWarps) * kSlots * 2 * kv_block_bytes(dim);
+  const size_t join = static_cast<size_t>(kWarps) * kRows * (dim * 4 + 8);
+  plan->smem = ring + join;
   return 0;
 }
 
@@ -729,33 +878,30 @@ int launch_kv(void (*kernel)(A...), dim3 grid, size_t smem, cudaStream_t stream,
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <int NG, int NT, bool kBf16>
+template <int NG, bool kBf16>
 int run_kv(const KvAttnParams& p, const KvPlan& plan, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (!(ready.load() >> dev & 1)) {
-    err = cudaFuncSetAttribute(kv_attn_kernel<NG, NT, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    err = cudaFuncSetAttribute(kv_attn_kernel<NG, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(plan.smem));
     if (err != cudaSuccess) return err;
     ready.fetch_or(1ull << dev);
   }
-  const dim3 grid(static_cast<unsigned>(plan.items), static_cast<unsigned>(p.kv_heads));
-  int rc = launch_kv(kv_attn_kernel<NG, NT, kBf16>, grid, plan.smem, stream, p);
+  const dim3 grid(static_cast<unsigned>(plan.ctas), static_cast<unsigned>(p.kv_heads));
+  int rc = launch_kv(kv_attn_kernel<NG, kBf16>, grid, plan.smem, stream, p);
   if (rc || !plan.combine) return rc;
-  // At most target / kv_heads + 1 runs share a (request, tile): the weights' room.
-  const size_t smem = 16 * kThreads + 4 * (static_cast<size_t>(plan.target / p.kv_heads) + 2);
-  return launch_kv(kv_combine_kernel<32 * NG, 8 * NT, kBf16>, grid, smem, stream, p);
+  return launch_kv(kv_combine_kernel<32 * NG, kBf16>, grid, 0, stream, p);
 }
 
 template <bool kBf16>
 int dispatch_kv(int dim, const KvAttnParams& p, const KvPlan& plan, cudaStream_t stream) {
-  const bool two = plan.tiles_nt == 2;
   switch (dim) {
-    case 64: return two ? run_kv<2, 2, kBf16>(p, plan, stream) : run_kv<2, 1, kBf16>(p, plan, stream);
-    case 128: return two ? run_kv<4, 2, kBf16>(p, plan, stream) : run_kv<4, 1, kBf16>(p, plan, stream);
-    default: return run_kv<8, 1, kBf16>(p, plan, stream);
+    case 64: return run_kv<2, kBf16>(p, plan, stream);
+    case 128: return run_kv<4, kBf16>(p, plan, stream);
+    default: return run_kv<8, kBf16>(p, plan, stream);
   }
 }
 
@@ -780,6 +926,7 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
   if (!q || !pages || !table || !lengths || !starts || !out || !scratch || tokens <= 0 || num_pages <= 0)
     return KLAB_E_INVALID;
   if (dtype != KLAB_DT_BF16 && dtype != KLAB_DT_F16) return KLAB_E_UNSUPPORTED;
+  if (!(scale > 0.0f) || scale > 3.0e38f) return KLAB_E_INVALID;
   KvPlan plan{};
   const int rc = kv_plan(requests, width, page_size, heads, kv_heads, dim, max_new, &plan);
   if (rc) return rc;
@@ -796,7 +943,7 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
   p.lengths = lengths;
   p.starts = starts;
   p.out = static_cast<unsigned short*>(out);
-  p.headers = reinterpret_cast<RunHeader*>(base + plan.headers);
+  p.headers = reinterpret_cast<Header*>(base + plan.headers);
   p.stats = reinterpret_cast<float2*>(base + plan.stats);
   p.sums = reinterpret_cast<float*>(base + plan.sums);
   p.status = device_status_address();
@@ -809,8 +956,10 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
   p.heads = heads;
   p.kv_heads = kv_heads;
   p.group = heads / kv_heads;
+  p.group_div = (65536 + p.group - 1) / p.group;
+  p.max_length = width * page_size;
+  p.whole = plan.whole;
   p.max_new = max_new;
-  p.target = plan.target;
   p.scale_log2e = scale * 1.44269504088896340736f;
   return dtype == KLAB_DT_BF16 ? dispatch_kv<true>(dim, p, plan, static_cast<cudaStream_t>(stream))
                                : dispatch_kv<false>(dim, p, plan, static_cast<cudaStream_t>(stream));

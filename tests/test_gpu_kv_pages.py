@@ -230,23 +230,32 @@ def test_offsets_past_32_bits():
 def close(out, q, starts, lengths, new, k, v, dtype, scale=None):
     """out's rows against the oracle over the quantised rows k, v (all requests behind one another).
 
-    Bounds per element, with A = sum of softmax * |v|: the FP16 rounding of p and of p * scale, 2^-11 each, give
-    2^-10 A; scores are exact but for FP32 sums (below 2^-15 in the exponent at these sizes), exp2 2^-22 and the FP32
-    sums of up to length / 16 products, together below 2^-13 A; weights under FP16's normal range add less than
-    2^-20 of the largest |v|; then half a step of the output type.
+    Bounds per element, with A = sum of softmax * |v| and M = sum of softmax * scale_G, for a value scale_G * (u - 8) with
+    u <= 15: the FP16 rounding of p and of p * scale, 2^-11 each at most and alike for u and for 8, give 2^-10 A; exp2 and
+    the FP32 weights and their sum, 2^-13 A; weights under FP16's normal range add less than 2^-20 of the largest |v|; then
+    half a step of the output type. The sums run over P' u and 8 P' apart, so their FP32 accumulators hold up to 23 M and take
+    at most length / 16 + 8 truncated additions of 2^-23 each. A score's group of 32 dims is
+    scale_G * (sum q u - 8 sum q): its FP32 accumulator holds at most 23 sum |q| and takes four truncated additions (two
+    MMAs, 2^-23 each at most, and the start and the scaled sum), so the score is off by at most
+    d = 4 * 2^-23 * 23 * scale * sum_G scale_G sum |q| and a weight, numerator and denominator, by 2 d.
     """
     scale = q.shape[2] ** -0.5 if scale is None else scale
     half = torch.finfo(DT[dtype]).eps / 2
     at = 0
     for s, length, n in zip(starts, lengths, new):
-        kk, vv = (ok.values(*ok.quantize(f64(x[at:at + length]))) for x in (k, v))
+        (kc, ks), (vc, vs) = (ok.quantize(f64(x[at:at + length])) for x in (k, v))
+        kk, vv = ok.values(kc, ks), ok.values(vc, vs)
         at += length
-        if not n:
+        if not n or not length:
             continue
         want, size = ok.attention(f64(q[s:s + n]), kk, vv, n, scale)
+        mass, _ = ok.attention(f64(q[s:s + n]), kk, np.repeat(vs, 32, -1), n, scale)
         got = f64(out[s:s + n])
         top = np.abs(vv).max(initial=0.0)
-        tol = half * np.abs(want) + (1 + half) * ((2.0 ** -10 + 2.0 ** -13) * size + 2.0 ** -20 * top) + 2.0 ** -24
+        qs = np.abs(f64(q[s:s + n])).reshape(n, ks.shape[1], -1, ks.shape[2], 32).sum(-1)
+        d = 92 * 2.0 ** -23 * scale * np.einsum("nhgG,hG->nhg", qs, ks.max(0)).reshape(n, -1, 1)
+        tol = half * np.abs(want) + (1 + half) * ((2.0 ** -10 + 2.0 ** -13 + 2 * d) * size + 2.0 ** -20 * top
+                                                 + (length / 16 + 8) * 23 * 2.0 ** -23 * mass) + 2.0 ** -24
         assert np.isfinite(got).all()
         worst = np.max(np.abs(got - want) - tol)
         assert worst <= 0, (length, n, worst)

@@ -20,12 +20,13 @@ scale per 32 dims of a token and head (include/klab_b200.h gives the format, csr
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
 
 from . import _native
-from ._module import get_module
+from ._launch import launch, ready
 
 HEAD_DIMS = (64, 128, 256)
 GROUP = 32            # dims that share a scale
@@ -71,13 +72,14 @@ def _check_page_size(page_size):
 
 def _check_ints(device, **tensors):
     for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device:
             raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
 
 
 def _check_device(device, *tensors):
-    if any(t.requires_grad for t in tensors):
-        raise ValueError("Inference only: no requires_grad")
+    for t in tensors:
+        if t.requires_grad:
+            raise ValueError("Inference only: no requires_grad")
     if device.type != "cuda":
         raise ValueError("Expected CUDA tensors")
 
@@ -123,26 +125,22 @@ def build_step(new_tokens, lengths, table, free_pages, free_count, *, page_size,
     state = (new_tokens, lengths, free_pages, free_count)
     _disjoint((table,), state)
     _check_device(device)
-    get_module(device)
     if inplace:
         _disjoint((lengths, free_count), state)
-        slots, positions, rows, starts, result = torch.empty(
-            3 * max_tokens + requests + 2, device=device, dtype=torch.int32).split(
-                (max_tokens, max_tokens, max_tokens, requests + 1, 1))
+    index = ready(device)
+    sizes = (max_tokens, max_tokens, max_tokens, requests + 1, 1)
+    if inplace:
+        slots, positions, rows, starts, result = torch.empty(sum(sizes), device=device, dtype=torch.int32).split(sizes)
         lengths_out, count_out = lengths, free_count
     else:
-        slots, positions, rows, starts, lengths_out, count_out, result = torch.empty(
-            3 * max_tokens + 2 * requests + 3, device=device, dtype=torch.int32).split(
-                (max_tokens, max_tokens, max_tokens, requests + 1, requests, 1, 1))
-    stream = torch.cuda.current_stream(device)
-    with torch.cuda.device(device):
-        rc = _native.lib().klab_kv_build_step(
-            new_tokens.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+        sizes += (requests, 1)
+        slots, positions, rows, starts, result, lengths_out, count_out = torch.empty(
+            sum(sizes), device=device, dtype=torch.int32).split(sizes)
+    launch("klab_kv_build_step", index,
+           (new_tokens.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
             requests, width, free_pages.numel(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
-            rows.data_ptr(), starts.data_ptr(), lengths_out.data_ptr(), count_out.data_ptr(), result.data_ptr(),
-            stream.cuda_stream)
-    _native.check(rc, "klab_kv_build_step")
-    _native.record(stream, *state, table, slots)
+            rows.data_ptr(), starts.data_ptr(), lengths_out.data_ptr(), count_out.data_ptr(), result.data_ptr()),
+           (*state, table))
     return BatchStep(slots, positions, rows, starts, lengths_out, count_out, result)
 
 
@@ -156,21 +154,16 @@ def release(ended, lengths, table, free_pages, free_count, *, page_size) -> None
     state = (ended, lengths, table, free_pages, free_count)
     _disjoint((lengths, table, free_pages, free_count), state)
     _check_device(device)
-    get_module(device)
-    stream = torch.cuda.current_stream(device)
-    with torch.cuda.device(device):
-        rc = _native.lib().klab_kv_release(ended.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(),
-                                           free_count.data_ptr(), table.shape[0], table.shape[1], free_pages.numel(),
-                                           page_size, stream.cuda_stream)
-    _native.check(rc, "klab_kv_release")
-    _native.record(stream, *state)
+    launch("klab_kv_release", ready(device),
+           (ended.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+            table.shape[0], table.shape[1], free_pages.numel(), page_size), state)
 
 
 def _check_pages(pages, head_dim):
     """(num_pages, kv_heads, page_size) of a pages tensor for heads of head_dim."""
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
-    if pages.dtype != torch.uint8 or pages.ndim != 3 or not pages.is_contiguous() or pages.data_ptr() % 16:
+    if pages.dtype is not torch.uint8 or pages.ndim != 3 or not pages.is_contiguous() or pages.data_ptr() % 16:
         raise ValueError("pages must be a contiguous, 16-byte aligned uint8 tensor [num_pages, kv_heads, page_bytes]")
     num_pages, kv_heads, size = pages.shape
     page_size = size * 8 // (9 * head_dim)
@@ -203,16 +196,14 @@ def store(k, v, pages, slots) -> None:
                 or x.data_ptr() % 8:
             raise ValueError("k and v need contiguous dims, strides of multiples of 4 and 8-byte alignment on the pages' device")
     _disjoint((pages,), (k, v, slots))
-    strides = [n if size > 1 else 0 for size, *both in ((tokens, k.stride(0), v.stride(0)), (heads, k.stride(1), v.stride(1)))
-               for n in both]
+    ks, kh, vs, vh = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    if tokens == 1 or heads == 1:  # a stride that is never taken may be anything
+        ks, vs = (ks, vs) if tokens > 1 else (0, 0)
+        kh, vh = (kh, vh) if heads > 1 else (0, 0)
     _check_device(device, k, v)
-    get_module(device)
-    stream = torch.cuda.current_stream(device)
-    with torch.cuda.device(device):
-        rc = _native.lib().klab_kv_store(k.data_ptr(), v.data_ptr(), _DT[k.dtype], *strides, pages.data_ptr(), slots.data_ptr(), tokens, num_pages, page_size,
-                                         kv_heads, dim, stream.cuda_stream)
-    _native.check(rc, "klab_kv_store")
-    _native.record(stream, k, v, pages, slots)
+    launch("klab_kv_store", ready(device),
+           (k.data_ptr(), v.data_ptr(), _DT[k.dtype], ks, vs, kh, vh, pages.data_ptr(), slots.data_ptr(), tokens, num_pages,
+            page_size, kv_heads, dim), (k, v, pages, slots))
 
 
 def read(pages, slots, head_dim, dtype=torch.bfloat16):
@@ -227,15 +218,23 @@ def read(pages, slots, head_dim, dtype=torch.bfloat16):
     if tokens * kv_heads * head_dim >= 2 ** 31:
         raise ValueError("Too many values for one call")
     _check_device(device)
-    get_module(device)
-    k, v = (torch.empty((tokens, kv_heads, head_dim), device=device, dtype=dtype) for _ in range(2))
-    stream = torch.cuda.current_stream(device)
-    with torch.cuda.device(device):
-        rc = _native.lib().klab_kv_read(pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _ODT[dtype], tokens,
-                                        num_pages, page_size, kv_heads, head_dim, stream.cuda_stream)
-    _native.check(rc, "klab_kv_read")
-    _native.record(stream, pages, slots)
+    index = ready(device)
+    k = torch.empty((tokens, kv_heads, head_dim), device=device, dtype=dtype)
+    v = torch.empty_like(k)
+    launch("klab_kv_read", index,
+           (pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _ODT[dtype], tokens, num_pages, page_size,
+            kv_heads, head_dim), (pages, slots))
     return k, v
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(index, *shape):
+    """klab_kv_attention_scratch of these shapes on device `index` (the grid depends on its SM count)."""
+    with torch.cuda.device(index):
+        need = _native.lib().klab_kv_attention_scratch(*shape)
+    if need < 0:
+        _native.check(int(need), "klab_kv_attention_scratch")
+    return int(need)
 
 
 def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=None):
@@ -274,21 +273,15 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
             raise ValueError("out must be contiguous, 16-byte aligned, of q's shape, dtype and device")
         _disjoint((out,), (q, pages, table, lengths, starts))
     _check_device(device, q)
-    get_module(device)
+    index = ready(device)
     if out is None:
-        out = torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
-    lib = _native.lib()
-    stream = torch.cuda.current_stream(device)
-    with torch.cuda.device(device):
-        need = lib.klab_kv_attention_scratch(requests, width, page_size, heads, kv_heads, dim, max_new)
-        if need < 0:
-            _native.check(int(need), "klab_kv_attention_scratch")
-        # Of this call alone: a captured graph keeps its own, and nothing has to be zero in it.
-        scratch = torch.empty(need, device=device, dtype=torch.uint8)
-        rc = lib.klab_kv_attention(q.data_ptr(), q.stride(0) if tokens > 1 else 0, _DT[q.dtype], pages.data_ptr(),
-                                   table.data_ptr(), lengths.data_ptr(), starts.data_ptr(), out.data_ptr(),
-                                   scratch.data_ptr(), need, tokens, requests, width, num_pages, page_size, heads, kv_heads,
-                                   dim, max_new, scale, stream.cuda_stream)
-    _native.check(rc, "klab_kv_attention")
-    _native.record(stream, q, pages, table, lengths, starts, out)
+        # q may be a slice of a wider row; out is not.
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
+    # Scratch of this call alone: a captured graph keeps its own, and nothing has to be zero in it.
+    need = _scratch_bytes(index, requests, width, page_size, heads, kv_heads, dim, max_new)
+    scratch = torch.empty(need, device=device, dtype=torch.uint8)
+    launch("klab_kv_attention", index,
+           (q.data_ptr(), q.stride(0) if tokens > 1 else 0, _DT[q.dtype], pages.data_ptr(), table.data_ptr(),
+            lengths.data_ptr(), starts.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, tokens, requests, width,
+            num_pages, page_size, heads, kv_heads, dim, max_new, scale), (q, pages, table, lengths, starts, out))
     return out

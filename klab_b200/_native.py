@@ -64,7 +64,7 @@ _SIGNATURES = {
     "klab_kv_attention": (_I, [_P, ct.c_longlong, _I] + [_P] * 6 + [ct.c_longlong] + [_I] * 9 + [ct.c_float, _P]),
     "klab_kv_attention_scratch": (ct.c_longlong, [_I] * 7),
     "klab_adapter_linear": (_I, [_I] + [_P] * 8 + [_I] * 6 + [_P, ct.c_longlong, _P, _SZ, _P]),
-    "klab_adapter_scratch": (ct.c_longlong, [_I] * 3),
+    "klab_adapter_scratch": (ct.c_longlong, [_I] * 5),
     "klab_add_rmsnorm_linear": (_I, [_P, _P, _P, ct.c_float, _P, _P, _P, _I, _I, _I, _P, _SZ, _P]),
     "klab_silu_mul_linear": (_I, [_P, _P, _P, _I, _I, _I, _P, _SZ, _P]),
     "klab_int8_linear": (_I, [_P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P, _SZ, _P]),

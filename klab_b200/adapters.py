@@ -11,15 +11,40 @@ reference, whose projections serve one set of weights.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _native
-from ._module import get_module
+from ._launch import launch, ready
 from .compressed_bf16 import PackedBF16
 from .fp4 import FP4F16Weights
 from .int8_weights import Int8Weights
 
 MAX_RANK = 256
+
+
+# Formats whose projection runs inside the adapters' own kernel (16-byte aligned rows); the others call the projection.
+_STREAMED = (_native.W_BF16, _native.W_I8_ROW, _native.W_FP4_G32H)
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(index, *shape):
+    with torch.cuda.device(index):
+        need = _native.lib().klab_adapter_scratch(*shape)
+    if need < 0:
+        _native.check(int(need), "klab_adapter_scratch")
+    return int(need)
+
+
+def _workspace(index, device, wfmt, m, n, k):
+    """The projection's split-K workspace. A captured call gets its own: two graphs captured on one stream may be replayed
+    on two, and must not share tickets."""
+    need = int(_native.lib().klab_gemv_workspace_bytes(wfmt, m, n, k))
+    if torch.cuda.is_current_stream_capturing():
+        return (torch.zeros(need, device=device, dtype=torch.uint8), need) if need else (None, 0)
+    buffer = _native.WORKSPACES.get(index, torch.cuda.current_stream(device), need)
+    return (buffer, buffer.numel()) if buffer is not None else (None, 0)
 
 
 def _weights(w, k):
@@ -86,25 +111,17 @@ def adapter_linear(x, w, a, b, scales, ids, *, out=None, output_dtype=torch.bflo
             raise ValueError("out must not overlap the inputs")
     if device.type != "cuda":
         raise ValueError("Expected CUDA tensors")
-    get_module(device)
+    index = ready(device)
     if out is None:
         out = torch.empty((m, n), device=device, dtype=output_dtype)
-    lib = _native.lib()
-    stream = torch.cuda.current_stream(device)
-    need = lib.klab_adapter_scratch(m, n, rank)
+    need = _scratch_bytes(index, wfmt, m, n, k, rank)
     scratch = torch.empty(need, device=device, dtype=torch.uint8)
-    if torch.cuda.is_current_stream_capturing():
-        # A graph's own: two graphs captured on one stream may be replayed on two, and must not share tickets.
-        ws_bytes = lib.klab_gemv_workspace_bytes(wfmt, m, n, k)
-        workspace = torch.zeros(ws_bytes, device=device, dtype=torch.uint8) if ws_bytes else None
-        ws_ptr = workspace.data_ptr() if ws_bytes else None
-    else:
-        ws_ptr, ws_bytes = _native.workspace_for(wfmt, m, n, k, device.index, stream)
-    with torch.cuda.device(device):
-        rc = lib.klab_adapter_linear(wfmt, x.data_ptr(), weights.data_ptr(), None if side is None else side.data_ptr(),
-                                     a.data_ptr(), b.data_ptr(), scales.data_ptr(), ids.data_ptr(), out.data_ptr(),
-                                     _native.DT_F32 if output_dtype == torch.float32 else _native.DT_BF16, m, n, k, rank,
-                                     count, scratch.data_ptr(), need, ws_ptr, ws_bytes, stream.cuda_stream)
-    _native.check(rc, "klab_adapter_linear")
-    _native.record(stream, *read, out)
+    workspace, ws_bytes = None, 0
+    if wfmt not in _STREAMED or weights.data_ptr() % 16 or weights.stride(0) * weights.element_size() % 16:
+        workspace, ws_bytes = _workspace(index, device, wfmt, m, n, k)
+    launch("klab_adapter_linear", index,
+           (wfmt, x.data_ptr(), weights.data_ptr(), None if side is None else side.data_ptr(), a.data_ptr(), b.data_ptr(),
+            scales.data_ptr(), ids.data_ptr(), out.data_ptr(),
+            _native.DT_F32 if output_dtype is torch.float32 else _native.DT_BF16, m, n, k, rank, count, scratch.data_ptr(),
+            need, None if workspace is None else workspace.data_ptr(), ws_bytes), (*read, out))
     return out

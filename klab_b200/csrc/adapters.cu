@@ -2,9 +2,23 @@
 //   y[m] = x[m] W^T + c_a (x[m] A_a^T) B_a^T,  a = ids[m] (-1: x[m] W^T alone),
 // BF16 x, A [S, r, K], B [S, N, r]; W in any format that the projections take with BF16 x and one scale tensor.
 //
-// shrink_kernel: t[m, j] = c_a * x[m] . A_a[j] in FP32; a CTA takes one token and kRanks rows of its A, its threads share
-// K with 16-byte loads. The projection then runs as it is, with FP32 output, and expand_kernel adds t[m] . B_a[n] to it in
-// FP32 and rounds once. Every sum has a fixed order.
+// BF16, INT8 per-row and E2M1/FP16-per-32 weights with 16-byte rows: two launches.
+//   adapter_stream_kernel reads W and the tokens' A once, as one list of work: a block is 128 rows (8 warps x 16 rows) of W,
+//   or 8 groups of 16 rows of the tokens' A (token m's adapter against x, of which column m counts), and a unit is 128
+//   bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM, so any N and K and
+//   any number of adapters keep every SM reading to the end. A warp multiplies its 16 rows by up to 16 tokens on
+//   mma.m16n8k16 with FP32 sums: lane (g, t) loads 16 bytes of rows g and g + 8 straight into the A fragments (the k slots
+//   of an MMA may be any columns as long as x's are the same), eight loads ahead; x lies in shared memory in fragment
+//   order. BF16 weights meet BF16 x; INT8 codes and E2M1 values are exact in FP16 and meet x in FP16 times a power of two
+//   of the (token, window), E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block goes to
+//   scratch in FP32.
+//   adapter_join_kernel adds the shares of each block in order, forms t = c (x A^T) the same way, and writes
+//   y + t . B_a[n] with one rounding.
+// Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
+//
+// What bounds it: HBM, the bytes of W and of the distinct adapters.
+#include <atomic>
+#include <climits>
 #include <cstdint>
 
 #include "common.cuh"
@@ -112,6 +126,475 @@ __global__ void __launch_bounds__(kAdThreads) expand_kernel(const AdapterParams 
     static_cast<unsigned short*>(p.out)[at] = f32_to_bf16_rn(y);
 }
 
+// ---------------------------------------------------------------- streaming form
+
+enum AdKind : int { AD_BF16 = 0, AD_I8 = 1, AD_FP4 = 2 };
+
+constexpr int kAsWarps = 8;
+constexpr int kAsThreads = 32 * kAsWarps;
+constexpr int kAsRows = 16 * kAsWarps;   // rows of a block
+constexpr int kAsTokens = 16;            // tokens of a call's tile
+constexpr int kAsUnit = 128;             // bytes of a row in a unit: two 64-byte steps
+constexpr int kAsAhead = 4;              // steps whose loads are in flight (two 16-byte loads each)
+constexpr int kAsWindow = 48 * 1024;     // x in shared memory
+constexpr int kAsMinShare = 4;           // units of a share at least
+
+// Columns per 64-byte step and 16-byte x pieces (8 columns of a token) per lane and step.
+__host__ __device__ constexpr int as_cols(int kind) { return kind == AD_BF16 ? 32 : kind == AD_I8 ? 64 : 128; }
+__host__ __device__ constexpr int as_pieces(int kind) { return as_cols(kind) / 32; }
+
+struct StreamParams {
+  const unsigned short* x;
+  const unsigned char* w;
+  const void* side;      // INT8: FP32 [N]; E2M1: FP16 [N, K / 32]
+  const unsigned short* a;
+  const unsigned short* b;
+  const float* c;
+  const int* ids;
+  float* w_part;         // [tile][block][piece][token][128]
+  float* a_part;         // [tile][block][piece][128]
+  void* out;
+  int* status;
+  long long row_bytes;
+  int m, n, k, rank, adapters, ldo, out_f32;
+  int groups;                    // 16-row groups of an adapter's A
+  int a_blocks, w_blocks;        // per tile of 16 tokens
+  int a_units, w_units;          // units of a block
+  int share, a_pieces, w_pieces; // units of a CTA; most shares that meet in a block
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four INT8 codes as two FP16 pairs, exact: 0x6400 | (code + 128) is 1152 + code.
+__device__ __forceinline__ void i8_pairs(unsigned w, unsigned& lo, unsigned& hi) {
+  const unsigned u = w ^ 0x80808080u;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
+}
+
+// Words (lane t, i) -> (lane i, t) among the four lanes of a row: lane t's 16 bytes are group t, and leave it with word t of
+// each group.
+__device__ __forceinline__ void transpose_quad(uint4& v, int t) {
+  const bool odd = t & 1, high = t & 2;
+  unsigned s0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v.z : v.w, 1);
+  if (odd)
+    v.x = s0, v.z = s1;
+  else
+    v.y = s0, v.w = s1;
+  s0 = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, 2), s1 = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, 2);
+  if (high)
+    v.x = s0, v.y = s1;
+  else
+    v.z = s0, v.w = s1;
+}
+
+// One piece of a share: units [u0, u1) of a block of kind KIND, for this warp's 16 rows at `base` (nullptr: no rows), of
+// which `rows` exist. Sums of row g (+ 8) and tokens 2 t (+ 1) of each 8-token block end in `sum`.
+template <int KIND, int NB>
+__device__ __forceinline__ void stream_piece(const StreamParams& p, const unsigned char* base, long long row_bytes,
+                                             const unsigned short* scales, int rows, int u0, int u1, int token0,
+                                             unsigned char* xs, int* top, float (&sum)[NB][4], bool first) {
+  constexpr int P = as_pieces(KIND), COLS = as_cols(KIND);
+  constexpr int kStepBytes = P * NB * 512;               // x of one step
+  constexpr int kSteps = kAsWindow / kStepBytes / kAsAhead * kAsAhead;  // steps of a window
+  const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int s_end = 2 * u1;
+  const bool has0 = base && g < rows, has1 = base && g + 8 < rows;
+  const unsigned char* r0 = base + g * row_bytes + 16 * t;
+  const unsigned char* r1 = r0 + 8 * row_bytes;
+  const long long srow = p.k / 32;  // E2M1: scales of a row, four to a step
+  const bool scales_vec = (srow & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0;
+  uint4 w0[kAsAhead], w1[kAsAhead];
+  uint2 f0[KIND == AD_FP4 ? kAsAhead : 1], f1[KIND == AD_FP4 ? kAsAhead : 1];
+  auto load = [&](int s, int j) {
+    const long long at = 64ll * s;
+    const bool in = s < s_end && at + 16 * t < row_bytes;
+    w0[j] = in && has0 ? ldg128_stream(r0 + at) : make_uint4(0u, 0u, 0u, 0u);
+    w1[j] = in && has1 ? ldg128_stream(r1 + at) : make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (KIND == AD_FP4) {
+      if (scales_vec) {
+        const bool there = s < s_end && 4 * s < srow;
+        f0[j] = there && has0 ? __ldg(reinterpret_cast<const uint2*>(scales + g * srow + 4 * s)) : make_uint2(0u, 0u);
+        f1[j] = there && has1 ? __ldg(reinterpret_cast<const uint2*>(scales + (g + 8) * srow + 4 * s)) : make_uint2(0u, 0u);
+      } else {
+        unsigned short v[8] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (s < s_end && 4 * s + i < srow) {
+            if (has0) v[i] = __ldg(scales + g * srow + 4 * s + i);
+            if (has1) v[4 + i] = __ldg(scales + (g + 8) * srow + 4 * s + i);
+          }
+        f0[j] = make_uint2(v[0] | static_cast<unsigned>(v[1]) << 16, v[2] | static_cast<unsigned>(v[3]) << 16);
+        f1[j] = make_uint2(v[4] | static_cast<unsigned>(v[5]) << 16, v[6] | static_cast<unsigned>(v[7]) << 16);
+      }
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kAsAhead; ++j) load(2 * u0 + j, j);
+  if (first) {  // the first weights are asked for before the previous kernel has ended
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
+  for (int s0 = 2 * u0; s0 < s_end; s0 += kSteps) {
+    const int steps = min(kSteps, s_end - s0);
+    // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t)
+    __syncthreads();  // the last window is read
+    if (KIND != AD_BF16 && tid < kAsTokens) top[tid] = 0;
+    if (KIND != AD_BF16) __syncthreads();
+    const int pieces = steps * P * NB * 32;
+    auto column = [&](int i) {
+      const int ln = i & 31, piece = (i >> 5) / NB % P, s = (i >> 5) / (NB * P);
+      return COLS * (s0 + s) + (KIND == AD_I8 ? 16 * (ln & 3) + 8 * piece : 32 * piece + 8 * (ln & 3));
+    };
+    auto fetch = [&](int i) {
+      const int token = token0 + (i >> 5) % NB * 8 + ((i & 31) >> 2), col = column(i);
+      return token < p.m && col < p.k
+                 ? __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token) * p.k + col))
+                 : make_uint4(0u, 0u, 0u, 0u);
+    };
+#pragma unroll 4
+    for (int i = tid; i < pieces; i += kAsThreads) {
+      const uint4 v = fetch(i);
+      if constexpr (KIND != AD_BF16) {  // the largest exponent of the token in the window
+        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+        unsigned most = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = __vmaxu2(most, (u[e] >> 7) & 0x00ff00ffu);
+        int ef = max(most & 0xffffu, most >> 16);
+        ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 1));
+        ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 2));
+        if ((tid & 3) == 0) atomicMax(top + (i >> 5) % NB * 8 + ((i & 31) >> 2), ef);
+      }
+      reinterpret_cast<uint4*>(xs)[i] = v;
+    }
+    __syncthreads();
+    if constexpr (KIND != AD_BF16) {  // BF16 -> FP16 times 2^(141 - ef): the largest lands below 2^15
+      for (int i = tid; i < pieces; i += kAsThreads) {
+        const uint4 v = reinterpret_cast<uint4*>(xs)[i];
+        unsigned u[4] = {v.x, v.y, v.z, v.w};
+        const int ef = min(max(top[(i >> 5) % NB * 8 + ((i & 31) >> 2)], 15), 254);
+        const float by = __int_as_float((268 - ef) << 23);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = bf16lo(u[e]) * by, hi = bf16hi(u[e]) * by;
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[e]) : "f"(hi), "f"(lo));
+        }
+        reinterpret_cast<uint4*>(xs)[i] = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      __syncthreads();
+    }
+    // ---- the window's steps
+    float acc[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[b][e] = 0.0f;
+    const unsigned xa = smem_addr(xs) + 16 * lane;
+    for (int s = 0; s < steps; s += kAsAhead) {
+#pragma unroll
+      for (int j = 0; j < kAsAhead; ++j) {
+        uint4 v0 = w0[j], v1 = w1[j];
+        uint2 q0, q1;
+        if constexpr (KIND == AD_FP4) q0 = f0[j], q1 = f1[j];
+        load(s0 + s + j + kAsAhead, j);
+        if (s + j < steps) {  // uniform
+          const unsigned at = xa + (s + j) * kStepBytes;
+          if constexpr (KIND == AD_BF16) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint4 xv = lds128(at + b * 512);
+              const unsigned a0[4] = {v0.x, v1.x, v0.y, v1.y}, a1[4] = {v0.z, v1.z, v0.w, v1.w};
+              mma_bf16(acc[b], a0, xv.x, xv.y);
+              mma_bf16(acc[b], a1, xv.z, xv.w);
+            }
+          } else if constexpr (KIND == AD_I8) {
+            const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
+            uint4 xv[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) xv[b][i] = lds128(at + (i * NB + b) * 512);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              unsigned a[4];
+              i8_pairs(c0[i], a[0], a[2]);
+              i8_pairs(c1[i], a[1], a[3]);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                mma_f16(acc[b], a, i & 1 ? xv[b][i >> 1].z : xv[b][i >> 1].x, i & 1 ? xv[b][i >> 1].w : xv[b][i >> 1].y);
+            }
+          } else {
+            transpose_quad(v0, t);
+            transpose_quad(v1, t);
+            const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
+            const unsigned g0[2] = {q0.x, q0.y}, g1[2] = {q1.x, q1.y};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // group i of the step: columns 8 t .. 8 t + 7 of it
+              const unsigned a0[4] = {e2m1x2_to_f16x2(c0[i] & 0xffu), e2m1x2_to_f16x2(c1[i] & 0xffu),
+                                      e2m1x2_to_f16x2(c0[i] >> 8 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 8 & 0xffu)};
+              const unsigned a1[4] = {e2m1x2_to_f16x2(c0[i] >> 16 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 16 & 0xffu),
+                                      e2m1x2_to_f16x2(c0[i] >> 24), e2m1x2_to_f16x2(c1[i] >> 24)};
+              const float h0 = f16_to_f32(static_cast<unsigned short>(g0[i >> 1] >> (16 * (i & 1))));
+              const float h1 = f16_to_f32(static_cast<unsigned short>(g1[i >> 1] >> (16 * (i & 1))));
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                const uint4 xv = lds128(at + (i * NB + b) * 512);
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_f16(d, a0, xv.x, xv.y);
+                mma_f16(d, a1, xv.z, xv.w);
+                acc[b][0] = fma_rn(d[0], h0, acc[b][0]), acc[b][1] = fma_rn(d[1], h0, acc[b][1]);
+                acc[b][2] = fma_rn(d[2], h1, acc[b][2]), acc[b][3] = fma_rn(d[3], h1, acc[b][3]);
+              }
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (KIND == AD_BF16) {
+          sum[b][e] += acc[b][e];
+        } else {
+          const int ef = min(max(top[8 * b + 2 * t + (e & 1)], 15), 254);
+          sum[b][e] = fma_rn(acc[b][e], __int_as_float((ef - 14) << 23), sum[b][e]);
+        }
+      }
+  }
+}
+
+template <int KIND, int NB>
+__global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const StreamParams p) {
+  extern __shared__ __align__(128) unsigned char xs[];
+  __shared__ int top[kAsTokens];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int tile = blockIdx.y, token0 = tile * kAsTokens;
+  const int a_total = p.a_blocks * p.a_units, total = a_total + p.w_blocks * p.w_units;
+  int pos = min(static_cast<long long>(blockIdx.x) * p.share, static_cast<long long>(total));
+  const int end = min(pos + p.share, total);
+  bool first = true;
+  while (pos < end) {
+    const bool is_a = pos < a_total;
+    const int units = is_a ? p.a_units : p.w_units, from = is_a ? 0 : a_total;
+    const int block = (pos - from) / units, u0 = pos - from - block * units, u1 = min(units, u0 + end - pos);
+    const int begin = from + block * units, piece = blockIdx.x - begin / p.share;
+    float sum[NB][4];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[b][e] = 0.0f;
+    if (is_a) {
+      if (first) {  // ids belong to the call, the weights below depend on them
+        grid_dependency_wait();
+        grid_launch_dependents();
+        first = false;
+      }
+      const int group = block * kAsWarps + warp, token = token0 + group / p.groups, rg = group % p.groups;
+      const bool there = group < kAsTokens * p.groups && token < p.m;
+      const int id = there ? __ldg(p.ids + token) : -1;
+      const bool has = id >= 0 && id < p.adapters;
+      if (there && !has && id != -1 && lane == 0) record_status(p.status, kStatusBadAdapter);
+      const unsigned char* base = has ? reinterpret_cast<const unsigned char*>(
+                                            p.a + (static_cast<long long>(id) * p.rank + 16 * rg) * p.k)
+                                      : nullptr;
+      stream_piece<AD_BF16, NB>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1, token0, xs, top, sum, false);
+      if (has) {
+        const int column = token - token0;
+        float* to = p.a_part + ((static_cast<long long>(tile) * p.a_blocks + block) * p.a_pieces + piece) * kAsRows + 16 * warp;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * b + 2 * t + (e & 1) == column) to[g + (e & 2 ? 8 : 0)] = sum[b][e];
+      }
+    } else {
+      const int row0 = block * kAsRows + 16 * warp, rows = p.n - row0;
+      const unsigned short* scales =
+          KIND == AD_FP4 ? static_cast<const unsigned short*>(p.side) + static_cast<long long>(row0) * (p.k / 32) : nullptr;
+      stream_piece<KIND, NB>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes, scales, rows, u0, u1, token0, xs,
+                             top, sum, first);
+      first = false;
+      const int tokens = min(kAsTokens, p.m - token0);
+      float* to = p.w_part + (((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces + piece) * kAsTokens) * kAsRows +
+                  16 * warp;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int token = 8 * b + 2 * t + (e & 1);
+          if (token < tokens) to[token * kAsRows + g + (e & 2 ? 8 : 0)] = sum[b][e];
+        }
+    }
+    pos += u1 - u0;
+  }
+}
+
+// 128 rows x 4 tokens of the result: one thread per row.
+constexpr int kJoinTokens = 4;
+template <int KIND>
+__global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParams p) {
+  __shared__ float ts[kJoinTokens][kMaxRank];
+  __shared__ int ids[kJoinTokens];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int tid = threadIdx.x, block = blockIdx.x, row = block * kAsRows + tid;
+  const int tile = blockIdx.y / (kAsTokens / kJoinTokens), first = blockIdx.y % (kAsTokens / kJoinTokens) * kJoinTokens;
+  const int token0 = tile * kAsTokens + first, tokens = min(kJoinTokens, p.m - token0);
+  if (tokens <= 0) return;
+  const int a_total = p.a_blocks * p.a_units;
+  if (tid < tokens) {
+    const int id = __ldg(p.ids + token0 + tid);
+    ids[tid] = id >= 0 && id < p.adapters ? id : -1;
+  }
+  // The shares of the block, in order.
+  const int begin = a_total + block * p.w_units;
+  const int pieces = (begin + p.w_units - 1) / p.share - begin / p.share + 1;
+  const float* from = p.w_part + ((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces * kAsTokens + first) * kAsRows + tid;
+  float y[kJoinTokens] = {};
+#pragma unroll 4
+  for (int q = 0; q < pieces; ++q)
+#pragma unroll
+    for (int j = 0; j < kJoinTokens; ++j)
+      if (j < tokens) y[j] += __ldcg(from + (static_cast<long long>(q) * kAsTokens + j) * kAsRows);
+  __syncthreads();
+  for (int i = tid; i < tokens * p.rank; i += kAsRows) {
+    const int j = i / p.rank, r = i - j * p.rank;
+    if (ids[j] < 0) continue;
+    const int group = (first + j) * p.groups + r / 16, ablock = group / kAsWarps;
+    const int abegin = ablock * p.a_units, apieces = (abegin + p.a_units - 1) / p.share - abegin / p.share + 1;
+    const float* src = p.a_part + (static_cast<long long>(tile) * p.a_blocks + ablock) * p.a_pieces * kAsRows +
+                       16 * (group % kAsWarps) + r % 16;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int q = 0; q < apieces; ++q) v += __ldcg(src + static_cast<long long>(q) * kAsRows);
+    ts[j][r] = mul_rn(v, __ldg(p.c + ids[j]));
+  }
+  __syncthreads();
+  if (row >= p.n) return;
+  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + row) : 1.0f;
+#pragma unroll
+  for (int j = 0; j < kJoinTokens; ++j) {
+    if (j >= tokens) break;
+    float v = KIND == AD_I8 ? mul_rn(y[j], scale) : y[j];
+    if (ids[j] >= 0) {
+      const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(ids[j]) * p.n + row) * p.rank);
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll 8
+      for (int r = 0; r < p.rank / 8; ++r) {
+        const uint4 w = __ldg(b + r);
+        const float* tj = ts[j] + 8 * r;
+        s0 = fma_rn(tj[0], bf16lo(w.x), s0), s1 = fma_rn(tj[1], bf16hi(w.x), s1);
+        s0 = fma_rn(tj[2], bf16lo(w.y), s0), s1 = fma_rn(tj[3], bf16hi(w.y), s1);
+        s0 = fma_rn(tj[4], bf16lo(w.z), s0), s1 = fma_rn(tj[5], bf16hi(w.z), s1);
+        s0 = fma_rn(tj[6], bf16lo(w.w), s0), s1 = fma_rn(tj[7], bf16hi(w.w), s1);
+      }
+      v = add_rn(v, add_rn(s0, s1));
+    }
+    const long long at = static_cast<long long>(token0 + j) * p.ldo + row;
+    if (p.out_f32)
+      static_cast<float*>(p.out)[at] = v;
+    else
+      static_cast<unsigned short*>(p.out)[at] = f32_to_bf16_rn(v);
+  }
+}
+
+struct StreamPlan {
+  int ctas, tiles;
+  size_t a_part, total;
+};
+
+bool stream_kind(int wfmt, int* kind) {
+  if (wfmt == KLAB_W_BF16) return *kind = AD_BF16, true;
+  if (wfmt == KLAB_W_I8_ROW) return *kind = AD_I8, true;
+  if (wfmt == KLAB_W_FP4_G32H) return *kind = AD_FP4, true;
+  return false;
+}
+
+// Fills the shares of p (m, n, k, rank set) for `places` CTAs.
+StreamPlan plan_stream(int kind, StreamParams& p, int places) {
+  StreamPlan s{};
+  p.row_bytes = kind == AD_BF16 ? 2ll * p.k : kind == AD_I8 ? p.k : p.k / 2;
+  p.groups = (p.rank + 15) / 16;
+  s.tiles = (p.m + kAsTokens - 1) / kAsTokens;
+  const int tokens = p.m < kAsTokens ? p.m : kAsTokens;
+  p.a_blocks = (tokens * p.groups + kAsWarps - 1) / kAsWarps;
+  p.w_blocks = (p.n + kAsRows - 1) / kAsRows;
+  p.a_units = static_cast<int>((2ll * p.k + kAsUnit - 1) / kAsUnit);
+  p.w_units = static_cast<int>((p.row_bytes + kAsUnit - 1) / kAsUnit);
+  const long long total = static_cast<long long>(p.a_blocks) * p.a_units + static_cast<long long>(p.w_blocks) * p.w_units;
+  const long long share = (total + places - 1) / places;
+  p.share = static_cast<int>(share < kAsMinShare ? kAsMinShare : share);
+  s.ctas = static_cast<int>((total + p.share - 1) / p.share);
+  p.a_pieces = (p.a_units - 1) / p.share + 2;
+  p.w_pieces = (p.w_units - 1) / p.share + 2;
+  s.a_part = static_cast<size_t>(s.tiles) * p.w_blocks * p.w_pieces * kAsTokens * kAsRows * 4;
+  s.total = s.a_part + static_cast<size_t>(s.tiles) * p.a_blocks * p.a_pieces * kAsRows * 4;
+  return s;
+}
+
+template <typename Kernel>
+int launch_stream(Kernel kernel, dim3 grid, int threads, size_t smem, const StreamParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int KIND, int NB>
+int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t stream) {
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (!(ready.load() >> dev & 1)) {
+    err = cudaFuncSetAttribute(adapter_stream_kernel<KIND, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAsWindow);
+    if (err != cudaSuccess) return err;
+    ready.fetch_or(1ull << dev);
+  }
+  const int rc = launch_stream(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, kAsWindow, p, stream);
+  if (rc) return rc;
+  return launch_stream(adapter_join_kernel<KIND>, dim3(p.w_blocks, plan.tiles * (kAsTokens / kJoinTokens)), kAsRows, 0, p,
+                       stream);
+}
+
+int sm_count(int* sms) {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return KLAB_E_UNSUPPORTED;
+  int n = cached[dev].load();
+  if (!n) {
+    err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (err != cudaSuccess) return err;
+    cached[dev].store(n);
+  }
+  *sms = n;
+  return 0;
+}
+
 template <typename Kernel>
 int launch_adapter(Kernel kernel, dim3 grid, const AdapterParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
@@ -131,10 +614,18 @@ int launch_adapter(Kernel kernel, dim3 grid, const AdapterParams& p, cudaStream_
 
 extern "C" {
 
-KLAB_API long long klab_adapter_scratch(int m, int n, int rank) {
-  if (m <= 0 || n <= 0 || rank <= 0) return KLAB_E_INVALID;
-  const long long t = (static_cast<long long>(m) * rank * 4 + 127) / 128 * 128;
-  return t + static_cast<long long>(m) * n * 4;
+KLAB_API long long klab_adapter_scratch(int wfmt, int m, int n, int k, int rank) {
+  using namespace klab;
+  if (m <= 0 || n <= 0 || k <= 0 || rank <= 0) return KLAB_E_INVALID;
+  const long long plain = (static_cast<long long>(m) * rank * 4 + 127) / 128 * 128 + static_cast<long long>(m) * n * 4;
+  int kind = 0, sms = 0;
+  if (!stream_kind(wfmt, &kind)) return plain;
+  const int rc = sm_count(&sms);
+  if (rc) return rc < 0 ? rc : -rc;
+  StreamParams p{};
+  p.m = m, p.n = n, p.k = k, p.rank = rank;
+  const long long shares = static_cast<long long>(plan_stream(kind, p, 2 * sms).total);
+  return shares > plain ? shares : plain;  // rows that are not 16-byte aligned take the plain form
 }
 
 KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const void* aux, const void* a, const void* b,
@@ -152,7 +643,40 @@ KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const v
   const uintptr_t mis = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(a) |
                         reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(scratch);
   if (mis & 15) return KLAB_E_ALIGN;
-  if (scratch_bytes < klab_adapter_scratch(m, n, rank)) return KLAB_E_INVALID;
+  if (scratch_bytes < klab_adapter_scratch(wfmt, m, n, k, rank)) return KLAB_E_INVALID;
+  int kind = 0;
+  if (stream_kind(wfmt, &kind)) {
+    StreamParams q{};
+    q.m = m, q.n = n, q.k = k, q.rank = rank;
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc) return rc;
+    const StreamPlan plan = plan_stream(kind, q, 2 * sms);
+    if ((reinterpret_cast<uintptr_t>(w) & 15) == 0 && q.row_bytes % 16 == 0 && plan.tiles * (kAsTokens / kJoinTokens) <= 65535 &&
+        static_cast<long long>(q.a_blocks) * q.a_units + static_cast<long long>(q.w_blocks) * q.w_units < INT_MAX) {
+      if (kind != AD_BF16 && !aux) return KLAB_E_INVALID;
+      if (kind == AD_FP4 && k % 32) return KLAB_E_SHAPE;
+      q.x = static_cast<const unsigned short*>(x);
+      q.w = static_cast<const unsigned char*>(w);
+      q.side = aux;
+      q.a = static_cast<const unsigned short*>(a);
+      q.b = static_cast<const unsigned short*>(b);
+      q.c = c;
+      q.ids = ids;
+      q.w_part = static_cast<float*>(scratch);
+      q.a_part = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + plan.a_part);
+      q.out = out;
+      q.status = device_status_address();
+      q.adapters = adapters;
+      q.ldo = n;
+      q.out_f32 = out_dtype == KLAB_DT_F32;
+      const cudaStream_t s = static_cast<cudaStream_t>(stream);
+      const bool one = m <= 8;
+      if (kind == AD_BF16) return one ? run_stream<AD_BF16, 1>(q, plan, s) : run_stream<AD_BF16, 2>(q, plan, s);
+      if (kind == AD_I8) return one ? run_stream<AD_I8, 1>(q, plan, s) : run_stream<AD_I8, 2>(q, plan, s);
+      return one ? run_stream<AD_FP4, 1>(q, plan, s) : run_stream<AD_FP4, 2>(q, plan, s);
+    }
+  }
   AdapterParams p{};
   p.x = static_cast<const unsigned short*>(x);
   p.a = static_cast<const unsigned short*>(a);

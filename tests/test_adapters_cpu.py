@@ -17,7 +17,7 @@ def call(**k):
 
 def test_c_refusals():
     for bad in ({"x": None}, {"a": None}, {"c": None}, {"ids": None}, {"scratch": None}, {"m": 0}, {"rank": 0}, {"adapters": 0},
-                {"bytes": 2 * 8 * 4}):
+                {"bytes": 2 * 8 * 4, "wfmt": _native.W_CBF16}):
         assert call(**bad) == _native.E_INVALID, bad
     for bad in ({"rank": 12}, {"rank": 264}, {"k": 60}, {"m": 65536}):
         assert call(**bad) == _native.E_SHAPE, bad
@@ -26,7 +26,7 @@ def test_c_refusals():
     for bad in ({"wfmt": _native.W_F32}, {"wfmt": _native.W_FP4_G16E}, {"dt": _native.DT_F16}):
         assert call(**bad) == _native.E_UNSUPPORTED, bad
     scratch = _native.lib().klab_adapter_scratch
-    assert scratch(2, 32, 8) == 128 + 256 and scratch(0, 1, 8) == _native.E_INVALID
+    assert scratch(_native.W_CBF16, 2, 32, 64, 8) == 128 + 256 and scratch(_native.W_BF16, 0, 1, 64, 8) == _native.E_INVALID
 
 
 def test_arguments():

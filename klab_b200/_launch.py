@@ -14,8 +14,9 @@ from . import _native
 from ._module import get_module
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
-_capturing = torch.cuda.is_current_stream_capturing
+_current_device = torch._C._cuda_getDevice
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+_functions = {}
 _streams = {}
 _ready = set()
 
@@ -31,17 +32,19 @@ def ready(device):
     return index
 
 
+def _resolve(name):
+    fn = _functions[name] = getattr(_native.lib(), name)
+    return fn
+
+
 def _stream_object(index, raw):
-    key = (index, raw)
-    stream = _streams.get(key)
-    if stream is None:
-        stream = _streams[key] = torch.cuda.current_stream(index)
+    stream = _streams[index, raw] = torch.cuda.current_stream(index)
     return stream
 
 
 def launch(name, index, args, tensors):
     """lib().<name>(*args, stream) on device `index`'s current stream; `tensors` are recorded on it outside capture."""
-    fn = getattr(_native.lib(), name)
+    fn = _functions.get(name) or _resolve(name)
     raw = _raw_stream(index)
     if _current_device() == index:
         rc = fn(*args, raw)
@@ -53,6 +56,6 @@ def launch(name, index, args, tensors):
     if rc:
         _native.check(rc, name)
     if not capturing:
-        stream = _stream_object(index, raw)
+        stream = _streams.get((index, raw)) or _stream_object(index, raw)
         for t in tensors:
             t.record_stream(stream)

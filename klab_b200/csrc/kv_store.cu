@@ -1,14 +1,19 @@
 // Rows of keys and values into 4-bit pages (store) and back (read): the cache that kv_attn.cu reads. The layout and the
 // format are in kv_pages.cuh.
 //
-// Store: a thread takes 4 dims of one (token, kv head) of K and of V with one 8-byte load each; the 8 threads of a
-// group of 32 dims find max|x| by a butterfly, s = RN16(min(max / 7, 65504)), and each value's code is
-// clamp(RNE(x / s), -7, 7) + 8 with x / s the correctly rounded quotient, so the codes are those of the definition, ties
-// included (x has at most 11 significant bits and s 11, hence |x / s - (k + 1/2)| is 0 or above 2^-13, far beyond the
-// quotient's rounding). NaN counts as 0; an infinity takes the largest code. A slot of -1 is skipped.
+// Store: a thread takes 8 dims of one (token, kv head) of K and of V with one 16-byte load each; the 4 threads of a group
+// of 32 dims find max|x| on the 16-bit patterns, s = RN16(min(max / 7, 65504)), and each value's code is
+// clamp(RNE(x / s), -7, 7) + 8. The quotient: q = x r with r = RN(1 / s), then q += (x - q s) r. It is within an ulp of
+// x / s, and exact where x / s is a float, as the ties k + 1/2 are; x has at most 11 significant bits and s 11, so
+// |x / s - (k + 1/2)| is 0 or above 2^-13, and RNE(q) is RNE(x / s), ties included. Adding 1.5 * 2^23 + 8 rounds to the
+// nearest even whole number and leaves the code in the low bits. Groups whose scale is under FP16's normal range or at its
+// end, and those with NaN (counted as 0) or infinities (the largest code), are clamped first. A slot of -1 is skipped.
+// Lanes of two neighbouring tokens join their halves of the V words where their slots are a pair (all of a prompt but its
+// ends); other tokens write halves.
 // Read: the inverse, (code - 8) * s in FP32 (exact) and one rounding to the output's type; a slot of -1 gives zeros.
 //
-// What bounds them: the bytes, 4 in and 1.125 out per pair of values (store of 16-bit rows).
+// What bounds them: the bytes, 4 in and 1.125 out per pair of values (store of 16-bit rows), and about 100 instructions a
+// thread beside them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -34,39 +39,100 @@ struct RowParams {
   void* k_out;
   void* v_out;
   int* status;
-  unsigned threads;
-  int num_pages, kv_heads, dim, page_shift;
+  unsigned threads, tokens;
+  int num_pages, kv_heads, dim, page_shift, wide;
 };
 
+constexpr float kCodeMagic = 12582912.0f + 8.0f;  // 1.5 * 2^23 + 8: adding it leaves round(q) + 8 in the low bits
+// Sum over i < 8 of the other bits of 1.5 * 2^23, shifted by 4 i.
+constexpr unsigned kCodeExcess = 0x4b400000u + 0xb4000000u + 0x40000000u;
+
 template <bool kBf16>
-__device__ __forceinline__ void widen4(uint2 w, float (&x)[4]) {
-  if (kBf16) {
-    x[0] = bf16lo(w.x), x[1] = bf16hi(w.x), x[2] = bf16lo(w.y), x[3] = bf16hi(w.y);
-  } else {
-    x[0] = f16lo(w.x), x[1] = f16hi(w.x), x[2] = f16lo(w.y), x[3] = f16hi(w.y);
-  }
+__device__ __forceinline__ f2 widen2(unsigned w) {
+  return kBf16 ? f2{bf16lo(w), bf16hi(w)} : f2{f16lo(w), f16hi(w)};
 }
 
-// The 4 codes of x and, through `scale`, the group's FP16 scale. Called by all 8 lanes of the group.
-__device__ __forceinline__ unsigned short quantize4(float (&x)[4], unsigned short& scale) {
-  float top = 0.0f;
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  unsigned long long ra, rb, rd;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
+  f2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
+  return d;
+}
+
+// The 8 codes of the values in v and, through `scale`, the group's FP16 scale. Called by all 4 lanes of the group.
+template <bool kBf16>
+__device__ __forceinline__ unsigned quantize8(uint4 v, unsigned short& scale) {
+  const unsigned w[4] = {v.x, v.y, v.z, v.w};
+  constexpr unsigned kInf = kBf16 ? 0x7f80u : 0x7c00u;
+  unsigned most = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (x[e] != x[e]) x[e] = 0.0f;
-    top = fmaxf(top, fabsf(x[e]));
+  for (int i = 0; i < 4; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+  most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+  const unsigned bits = max(most & 0xffffu, most >> 16);
+  float top = kBf16 ? __uint_as_float(bits << 16) : f16_to_f32(static_cast<unsigned short>(bits));
+  f2 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = widen2<kBf16>(w[i]);
+  // Any lane with an odd group sends its warp through the full path, which gives ordinary groups the same codes.
+  if (__any_sync(0xffffffffu, bits >= kInf)) {
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (x[i].x != x[i].x) x[i].x = 0.0f;
+      if (x[i].y != x[i].y) x[i].y = 0.0f;
+      top = fmaxf(top, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   }
-#pragma unroll
-  for (int d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   const __half s16 = __float2half_rn(fminf(__fdiv_rn(top, 7.0f), 65504.0f));
   scale = __half_as_ushort(s16);
   const float s = __half2float(s16);
-  unsigned piece = 0;
+  if (s == 0.0f) return 0x88888888u;
+  if (s < 6.103515625e-5f || s >= 65504.0f) {  // x / s may pass 7
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float code = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -7.0f), 7.0f) : 0.0f;
-    piece |= static_cast<unsigned>(static_cast<int>(code) + 8) << (4 * e);
+    for (int i = 0; i < 4; ++i) {
+      x[i].x = fminf(fmaxf(x[i].x, -7.0f * s), 7.0f * s);
+      x[i].y = fminf(fmaxf(x[i].y, -7.0f * s), 7.0f * s);
+    }
   }
-  return static_cast<unsigned short>(piece);
+  const float r = __frcp_rn(s);
+  const f2 r2 = {r, r}, minus = {-s, -s}, magic = {kCodeMagic, kCodeMagic};
+  unsigned codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f2 q = mul2(x[i], r2);
+    q = fma2(fma2(q, minus, x[i]), r2, q);
+    q = add2(q, magic);
+    codes += __float_as_uint(q.x) << (8 * i);
+    codes += __float_as_uint(q.y) << (8 * i + 4);
+  }
+  return codes - kCodeExcess;
+}
+
+// Token, head and 8-dim run of a thread: runs, then the two tokens of a pair, then heads, then pairs.
+struct Place {
+  unsigned token;
+  int head, c, slot;
+  long long block;
+};
+
+__device__ __forceinline__ Place place_of(const RowParams& p, unsigned at) {
+  Place w;
+  const unsigned runs = p.dim / 8;  // a power of two
+  const int shift = 31 - __clz(static_cast<int>(runs));
+  w.c = at & (runs - 1);
+  const unsigned rest = at >> (shift + 1), pair = rest / p.kv_heads;
+  w.head = rest - pair * p.kv_heads;
+  w.token = 2 * pair + (at >> shift & 1);
+  w.slot = w.token < p.tokens ? p.slots[w.token] : -1;
+  w.block = kv_block_offset(w.slot, w.head, p.num_pages, p.kv_heads, p.page_shift, p.dim);
+  if (w.slot != -1 && w.block < 0) record_status(p.status, kStatusBadPage);
+  return w;
 }
 
 template <bool kBf16>
@@ -74,51 +140,72 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const RowParams
   grid_dependency_wait();
   grid_launch_dependents();
   const unsigned at = blockIdx.x * kStoreThreads + threadIdx.x;
-  const unsigned per_head = p.dim / 4, per_token = per_head * p.kv_heads;
-  const unsigned token = at / per_token, rest = at - token * per_token;
-  const int head = rest / per_head, c = rest - head * per_head;
-  // A thread past the end stays for the groups' butterflies.
-  const int slot = at < p.threads ? p.slots[token] : -1;
-  const long long block = kv_block_offset(slot, head, p.num_pages, p.kv_heads, p.page_shift, p.dim);
-  if (slot != -1 && block < 0) record_status(p.status, kStatusBadPage);
-  float k[4] = {}, v[4] = {};
-  if (block >= 0) {
-    const auto* ks = static_cast<const unsigned short*>(p.k) + token * p.k_stride + head * p.k_head + 4 * c;
-    const auto* vs = static_cast<const unsigned short*>(p.v) + token * p.v_stride + head * p.v_head + 4 * c;
-    widen4<kBf16>(__ldg(reinterpret_cast<const uint2*>(ks)), k);
-    widen4<kBf16>(__ldg(reinterpret_cast<const uint2*>(vs)), v);
+  const Place w = place_of(p, at);  // a thread past the end has a slot of -1 and stays for the shuffles
+  uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
+  if (w.block >= 0) {
+    const long long row = w.token;
+    const auto* ks = static_cast<const unsigned short*>(p.k) + row * p.k_stride + w.head * p.k_head + 8 * w.c;
+    const auto* vs = static_cast<const unsigned short*>(p.v) + row * p.v_stride + w.head * p.v_head + 8 * w.c;
+    if (p.wide) {
+      k = ldg128_stream(ks);
+      v = ldg128_stream(vs);
+    } else {  // rows on 8-byte boundaries
+      const uint2 k0 = __ldg(reinterpret_cast<const uint2*>(ks)), k1 = __ldg(reinterpret_cast<const uint2*>(ks) + 1);
+      const uint2 v0 = __ldg(reinterpret_cast<const uint2*>(vs)), v1 = __ldg(reinterpret_cast<const uint2*>(vs) + 1);
+      k = make_uint4(k0.x, k0.y, k1.x, k1.y);
+      v = make_uint4(v0.x, v0.y, v1.x, v1.y);
+    }
   }
   unsigned short k_scale, v_scale;
-  const unsigned short k_piece = quantize4(k, k_scale), v_piece = quantize4(v, v_scale);
-  if (block < 0) return;
-  unsigned short* to = p.pages + block / 2;
-  const int r = slot & (kKvBlock - 1);
-  to[kv_k_piece(r, c, p.dim)] = k_piece;
-  to[kv_v_piece(r, c, p.dim)] = v_piece;
-  if ((c & 7) == 0) {
-    to[kv_k_scale(r, c >> 3, p.dim)] = k_scale;
-    to[kv_v_scale(r, c >> 3, p.dim)] = v_scale;
+  const unsigned k_codes = quantize8<kBf16>(k, k_scale), v_codes = quantize8<kBf16>(v, v_scale);
+  // The other token of the pair: its V codes and slot (heads of 256 take a warp each and write halves).
+  const int other = p.dim / 8;
+  const unsigned v_other = __shfl_xor_sync(0xffffffffu, v_codes, other & 31);
+  const int slot_other = __shfl_xor_sync(0xffffffffu, w.slot, other & 31);
+  if (w.block < 0) return;
+  unsigned short* to = p.pages + w.block / 2;
+  const int r = w.slot & (kKvBlock - 1);
+  *reinterpret_cast<unsigned*>(to + kv_k_piece(r, 2 * w.c, p.dim)) = k_codes;
+  // Pieces 2 c and 2 c + 1 (dims 8 c .. + 3, 8 c + 4 .. + 7): neighbouring g of one group.
+  if (other < 32 && slot_other == (w.slot ^ 1)) {
+    if ((w.slot & 1) == 0)
+      *reinterpret_cast<unsigned*>(to + kv_v_piece(r, 2 * w.c, p.dim)) = __byte_perm(v_codes, v_other, 0x5410);
+    else
+      *reinterpret_cast<unsigned*>(to + kv_v_piece(r & ~1, 2 * w.c + 1, p.dim)) = __byte_perm(v_other, v_codes, 0x7632);
+  } else {
+    to[kv_v_piece(r, 2 * w.c, p.dim)] = static_cast<unsigned short>(v_codes);
+    to[kv_v_piece(r, 2 * w.c + 1, p.dim)] = static_cast<unsigned short>(v_codes >> 16);
+  }
+  if ((w.c & 3) == 0) {
+    to[kv_k_scale(r, w.c >> 2, p.dim)] = k_scale;
+    to[kv_v_scale(r, w.c >> 2, p.dim)] = v_scale;
   }
 }
 
 template <int kOut>
-__device__ __forceinline__ void put4(void* out, unsigned at, unsigned piece, float s) {
-  float x[4];
+__device__ __forceinline__ void put8(void* out, long long at, unsigned codes, float s) {
+  f2 x[4];
+  const f2 s2 = {s, s}, back = {-kCodeMagic, -kCodeMagic};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = static_cast<float>(static_cast<int>(piece >> (4 * e) & 15u) - 8) * s;
+  for (int i = 0; i < 4; ++i) {
+    const f2 u = {__uint_as_float((codes >> (8 * i) & 15u) | 0x4b400000u),
+                  __uint_as_float((codes >> (8 * i + 4) & 15u) | 0x4b400000u)};
+    x[i] = mul2(add2(u, back), s2);
+  }
   if (kOut == KLAB_DT_F32) {
-    reinterpret_cast<float4*>(out)[at] = make_float4(x[0], x[1], x[2], x[3]);
+    float4* to = reinterpret_cast<float4*>(out) + 2 * at;
+    to[0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+    to[1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
   } else {
-    unsigned w[2];
+    unsigned w[4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int i = 0; i < 4; ++i) {
       if (kOut == KLAB_DT_BF16)
-        w[e] = f32_to_bf16_rn(x[2 * e]) | static_cast<unsigned>(f32_to_bf16_rn(x[2 * e + 1])) << 16;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[i].y), "f"(x[i].x));
       else
-        w[e] = __half_as_ushort(__float2half_rn(x[2 * e])) |
-               static_cast<unsigned>(__half_as_ushort(__float2half_rn(x[2 * e + 1]))) << 16;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[i].y), "f"(x[i].x));
     }
-    reinterpret_cast<uint2*>(out)[at] = make_uint2(w[0], w[1]);
+    reinterpret_cast<uint4*>(out)[at] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -127,26 +214,21 @@ __global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const RowParams 
   grid_dependency_wait();
   grid_launch_dependents();
   const unsigned at = blockIdx.x * kStoreThreads + threadIdx.x;
-  if (at >= p.threads) return;
-  const unsigned per_head = p.dim / 4, per_token = per_head * p.kv_heads;
-  const unsigned token = at / per_token, rest = at - token * per_token;
-  const int head = rest / per_head, c = rest - head * per_head;
-  const int slot = p.slots[token];
-  const long long block = kv_block_offset(slot, head, p.num_pages, p.kv_heads, p.page_shift, p.dim);
-  unsigned k_piece = 0x8888u, v_piece = 0x8888u;
+  const Place w = place_of(p, at);
+  if (w.token >= p.tokens) return;
+  unsigned k_codes = 0x88888888u, v_codes = 0x88888888u;
   float k_scale = 0.0f, v_scale = 0.0f;
-  if (block >= 0) {
-    const unsigned short* from = p.pages + block / 2;
-    const int r = slot & (kKvBlock - 1);
-    k_piece = from[kv_k_piece(r, c, p.dim)];
-    v_piece = from[kv_v_piece(r, c, p.dim)];
-    k_scale = f16_to_f32(from[kv_k_scale(r, c >> 3, p.dim)]);
-    v_scale = f16_to_f32(from[kv_v_scale(r, c >> 3, p.dim)]);
-  } else if (slot != -1) {
-    record_status(p.status, kStatusBadPage);
+  if (w.block >= 0) {
+    const unsigned short* from = p.pages + w.block / 2;
+    const int r = w.slot & (kKvBlock - 1);
+    k_codes = *reinterpret_cast<const unsigned*>(from + kv_k_piece(r, 2 * w.c, p.dim));
+    v_codes = from[kv_v_piece(r, 2 * w.c, p.dim)] | static_cast<unsigned>(from[kv_v_piece(r, 2 * w.c + 1, p.dim)]) << 16;
+    k_scale = f16_to_f32(from[kv_k_scale(r, w.c >> 2, p.dim)]);
+    v_scale = f16_to_f32(from[kv_v_scale(r, w.c >> 2, p.dim)]);
   }
-  put4<kOut>(p.k_out, at, k_piece, k_scale);
-  put4<kOut>(p.v_out, at, v_piece, v_scale);
+  const long long to = (static_cast<long long>(w.token) * p.kv_heads + w.head) * (p.dim / 8) + w.c;
+  put8<kOut>(p.k_out, to, k_codes, k_scale);
+  put8<kOut>(p.v_out, to, v_codes, v_scale);
 }
 
 int check_pages(const void* pages, const void* slots, int tokens, int num_pages, int page_size, int kv_heads, int dim) {
@@ -203,11 +285,14 @@ KLAB_API int klab_kv_store(const void* k, const void* v, int dtype, long long k_
   p.v_stride = v_stride;
   p.k_head = k_head;
   p.v_head = v_head;
+  p.wide = !((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15 ||
+             (k_stride | v_stride | k_head | v_head) & 7);
   p.pages = static_cast<unsigned short*>(pages);
   p.slots = slots;
   p.status = device_status_address();
   p.num_pages = num_pages;
-  p.threads = static_cast<unsigned>(tokens) * kv_heads * (dim / 4);
+  p.tokens = static_cast<unsigned>(tokens);
+  p.threads = (p.tokens + 1) / 2 * 2 * kv_heads * (dim / 8);
   p.kv_heads = kv_heads;
   p.dim = dim;
   p.page_shift = kv_page_shift(page_size);
@@ -229,7 +314,8 @@ KLAB_API int klab_kv_read(const void* pages, const int* slots, void* k_out, void
   p.v_out = v_out;
   p.status = device_status_address();
   p.num_pages = num_pages;
-  p.threads = static_cast<unsigned>(tokens) * kv_heads * (dim / 4);
+  p.tokens = static_cast<unsigned>(tokens);
+  p.threads = (p.tokens + 1) / 2 * 2 * kv_heads * (dim / 8);
   p.kv_heads = kv_heads;
   p.dim = dim;
   p.page_shift = kv_page_shift(page_size);

@@ -84,24 +84,43 @@ def _check_device(device, *tensors):
         raise ValueError("Expected CUDA tensors")
 
 
-def _disjoint(written, read):
-    for a in written:
-        a0, a1 = a.data_ptr(), a.data_ptr() + a.numel() * a.element_size()
-        for b in read:
-            b0 = b.data_ptr()
-            if a is not b and a0 < b0 + b.numel() * b.element_size() and b0 < a1:
+def _span(t):
+    """First and last byte + 1 that a tensor with positive strides reaches."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.numel() * t.element_size()
+    return p, p + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _disjoint(written, *read):
+    """`written` shares no byte with the others."""
+    w0, w1 = _span(written)
+    for t in read:
+        if t is not written:
+            r0, r1 = _span(t)
+            if r0 < w1 and w0 < r1:
                 raise ValueError("Tensors that are written must not overlap the others")
 
 
-def _check_state(lengths, table, free_pages, free_count, page_size):
+@lru_cache(maxsize=256, typed=True)
+def _check_sizes(page_size, lengths, table, free_pages, free_count):
+    """The shapes of a batch's state; cached, since a server's never change."""
     _check_page_size(page_size)
-    _check_ints(lengths.device, lengths=lengths, table=table, free_pages=free_pages, free_count=free_count)
-    if lengths.ndim != 1 or table.ndim != 2 or table.shape[0] != lengths.shape[0] or free_pages.ndim != 1 \
-            or free_count.numel() != 1 or min(table.shape) <= 0 or free_pages.numel() <= 0:
+    if len(lengths) != 1 or len(table) != 2 or table[0] != lengths[0] or len(free_pages) != 1 \
+            or math.prod(free_count) != 1 or min(table) <= 0 or free_pages[0] <= 0:
         raise ValueError("Expected lengths=[requests], table=[requests, width], free_pages=[num_pages], free_count=[1]")
-    if lengths.shape[0] > MAX_REQUESTS or free_pages.numel() * page_size >= 2 ** 31 \
-            or table.shape[1] * page_size >= 2 ** 31:
+    if lengths[0] > MAX_REQUESTS or free_pages[0] * page_size >= 2 ** 31 or table[1] * page_size >= 2 ** 31:
         raise ValueError(f"At most {MAX_REQUESTS} requests, and fewer than 2^31 slots and positions")
+    return table[0], table[1], free_pages[0]
+
+
+def _check_state(lengths, table, free_pages, free_count, page_size):
+    """(requests, width, num_pages) of a batch's state."""
+    _check_ints(lengths.device, lengths=lengths, table=table, free_pages=free_pages, free_count=free_count)
+    try:
+        return _check_sizes(page_size, lengths.shape, table.shape, free_pages.shape, free_count.shape)
+    except TypeError:
+        raise ValueError("page_size must be a power of two from 16 to 1024") from None
 
 
 def build_step(new_tokens, lengths, table, free_pages, free_count, *, page_size, max_tokens, inplace=False) -> BatchStep:
@@ -114,19 +133,18 @@ def build_step(new_tokens, lengths, table, free_pages, free_count, *, page_size,
     themselves, for a captured step). max_tokens bounds the step's tokens. All or nothing: where result is not STEP_OK,
     no page was given out and there are no tokens.
     """
-    _check_state(lengths, table, free_pages, free_count, page_size)
+    requests, width, num_pages = _check_state(lengths, table, free_pages, free_count, page_size)
     device = lengths.device
     _check_ints(device, new_tokens=new_tokens)
-    requests, width = table.shape
     if new_tokens.shape != lengths.shape:
         raise ValueError("new_tokens must have one entry per request")
     if not 0 < max_tokens < 2 ** 31:
         raise ValueError("max_tokens must be positive and below 2^31")
-    state = (new_tokens, lengths, free_pages, free_count)
-    _disjoint((table,), state)
-    _check_device(device)
+    _disjoint(table, new_tokens, lengths, free_pages, free_count)
     if inplace:
-        _disjoint((lengths, free_count), state)
+        _disjoint(lengths, new_tokens, free_pages, free_count)
+        _disjoint(free_count, new_tokens, free_pages)
+    _check_device(device)
     index = ready(device)
     sizes = (max_tokens, max_tokens, max_tokens, requests + 1, 1)
     if inplace:
@@ -138,34 +156,36 @@ def build_step(new_tokens, lengths, table, free_pages, free_count, *, page_size,
             sum(sizes), device=device, dtype=torch.int32).split(sizes)
     launch("klab_kv_build_step", index,
            (new_tokens.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-            requests, width, free_pages.numel(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
+            requests, width, num_pages, page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
             rows.data_ptr(), starts.data_ptr(), lengths_out.data_ptr(), count_out.data_ptr(), result.data_ptr()),
-           (*state, table))
+           (new_tokens, lengths, free_pages, free_count, table))
     return BatchStep(slots, positions, rows, starts, lengths_out, count_out, result)
 
 
 def release(ended, lengths, table, free_pages, free_count, *, page_size) -> None:
     """Requests with ended[i] (bool) give their pages back: pushed on the free stack, their table entries -1 and their
     lengths 0, all in place. Nothing changes (device status 4) when one of their table entries is no page."""
-    _check_state(lengths, table, free_pages, free_count, page_size)
+    requests, width, num_pages = _check_state(lengths, table, free_pages, free_count, page_size)
     device = lengths.device
     if ended.dtype != torch.bool or ended.device != device or ended.shape != lengths.shape or not ended.is_contiguous():
         raise ValueError("ended must be a contiguous bool tensor with one entry per request")
     state = (ended, lengths, table, free_pages, free_count)
-    _disjoint((lengths, table, free_pages, free_count), state)
+    for t in state[1:]:
+        _disjoint(t, *state)
     _check_device(device)
     launch("klab_kv_release", ready(device),
            (ended.data_ptr(), lengths.data_ptr(), table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-            table.shape[0], table.shape[1], free_pages.numel(), page_size), state)
+            requests, width, num_pages, page_size), state)
 
 
-def _check_pages(pages, head_dim):
-    """(num_pages, kv_heads, page_size) of a pages tensor for heads of head_dim."""
+@lru_cache(maxsize=256, typed=True)
+def _page_layout(shape, head_dim):
+    """(num_pages, kv_heads, page_size) of pages of this shape for heads of head_dim."""
     if head_dim not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
-    if pages.dtype is not torch.uint8 or pages.ndim != 3 or not pages.is_contiguous() or pages.data_ptr() % 16:
-        raise ValueError("pages must be a contiguous, 16-byte aligned uint8 tensor [num_pages, kv_heads, page_bytes]")
-    num_pages, kv_heads, size = pages.shape
+    if len(shape) != 3:
+        raise ValueError("pages must be [num_pages, kv_heads, page_bytes]")
+    num_pages, kv_heads, size = shape
     page_size = size * 8 // (9 * head_dim)
     if min(num_pages, kv_heads) <= 0 or page_size * head_dim * 9 != size * 8:
         raise ValueError("pages do not hold whole tokens of this head_dim (see page_bytes)")
@@ -175,35 +195,42 @@ def _check_pages(pages, head_dim):
     return num_pages, kv_heads, page_size
 
 
+def _check_pages(pages, head_dim):
+    layout = _page_layout(pages.shape, head_dim)
+    if pages.dtype is not torch.uint8 or not pages.is_contiguous() or pages.data_ptr() % 16:
+        raise ValueError("pages must be a contiguous, 16-byte aligned uint8 tensor [num_pages, kv_heads, page_bytes]")
+    return layout
+
+
 def store(k, v, pages, slots) -> None:
     """Rows k, v [tokens, kv_heads, head_dim] (BF16 or FP16; any token and head strides that are multiples of 4 elements,
     such as slices of a fused projection's output) into pages at slots [tokens] (int32). A slot of -1 is skipped; two
     tokens of one call must not name the same slot."""
-    if k.ndim != 3 or v.shape != k.shape or k.dtype not in _DT or v.dtype != k.dtype:
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or v.shape != shape or dtype not in _DT or v.dtype is not dtype:
         raise ValueError("Expected k and v [tokens, kv_heads, head_dim] in BF16 or FP16")
-    tokens, heads, dim = k.shape
+    tokens, heads, dim = shape
     num_pages, kv_heads, page_size = _check_pages(pages, dim)
     if heads != kv_heads or tokens <= 0:
         raise ValueError("k and v must have the pages' kv_heads and at least one token")
     if tokens * heads * dim >= 2 ** 31:
         raise ValueError("Too many values for one call")
     device = pages.device
-    _check_ints(device, slots=slots)
-    if slots.shape != (tokens,):
-        raise ValueError("slots must have one entry per token")
-    for x in (k, v):
-        if x.device != device or x.stride(2) != 1 or (tokens > 1 and x.stride(0) % 4) or (heads > 1 and x.stride(1) % 4) \
-                or x.data_ptr() % 8:
-            raise ValueError("k and v need contiguous dims, strides of multiples of 4 and 8-byte alignment on the pages' device")
-    _disjoint((pages,), (k, v, slots))
-    ks, kh, vs, vh = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    if slots.dtype is not torch.int32 or slots.shape != (tokens,) or not slots.is_contiguous() or slots.device != device:
+        raise ValueError(f"slots must be a contiguous int32 tensor with one entry per token on {device}")
+    ks, kh, kd = k.stride()
+    vs, vh, vd = v.stride()
     if tokens == 1 or heads == 1:  # a stride that is never taken may be anything
         ks, vs = (ks, vs) if tokens > 1 else (0, 0)
         kh, vh = (kh, vh) if heads > 1 else (0, 0)
+    kp, vp, pp = k.data_ptr(), v.data_ptr(), pages.data_ptr()
+    if kd != 1 or vd != 1 or (ks | vs | kh | vh) & 3 or (kp | vp) & 7 or k.device != device or v.device != device:
+        raise ValueError("k and v need contiguous dims, strides of multiples of 4 and 8-byte alignment on the pages' device")
+    _disjoint(pages, k, v, slots)
     _check_device(device, k, v)
     launch("klab_kv_store", ready(device),
-           (k.data_ptr(), v.data_ptr(), _DT[k.dtype], ks, vs, kh, vh, pages.data_ptr(), slots.data_ptr(), tokens, num_pages,
-            page_size, kv_heads, dim), (k, v, pages, slots))
+           (kp, vp, _DT[dtype], ks, vs, kh, vh, pp, slots.data_ptr(), tokens, num_pages, page_size, kv_heads, dim),
+           (k, v, pages, slots))
 
 
 def read(pages, slots, head_dim, dtype=torch.bfloat16):
@@ -211,15 +238,16 @@ def read(pages, slots, head_dim, dtype=torch.bfloat16):
     exact). Zeros for a slot of -1."""
     num_pages, kv_heads, page_size = _check_pages(pages, head_dim)
     device = pages.device
-    _check_ints(device, slots=slots)
     if dtype not in _ODT or slots.ndim != 1 or slots.numel() <= 0:
         raise ValueError("Expected slots=[tokens] and a dtype of float32, bfloat16 or float16")
+    if slots.dtype is not torch.int32 or not slots.is_contiguous() or slots.device != device:
+        raise ValueError(f"slots must be a contiguous int32 tensor on {device}")
     tokens = slots.numel()
     if tokens * kv_heads * head_dim >= 2 ** 31:
         raise ValueError("Too many values for one call")
     _check_device(device)
     index = ready(device)
-    k = torch.empty((tokens, kv_heads, head_dim), device=device, dtype=dtype)
+    k = torch.empty(tokens, kv_heads, head_dim, device=device, dtype=dtype)
     v = torch.empty_like(k)
     launch("klab_kv_read", index,
            (pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _ODT[dtype], tokens, num_pages, page_size,
@@ -245,43 +273,49 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
     below lengths[i] - n + j + 1, and a row that sees none gives zeros. scale defaults to 1 / sqrt(head_dim). Rows of q
     that belong to no request leave their rows of `out` as they were.
     """
-    if q.ndim != 3 or q.dtype not in _DT:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or dtype not in _DT:
         raise ValueError("Expected q [tokens, heads, head_dim] in BF16 or FP16")
-    tokens, heads, dim = q.shape
+    tokens, heads, dim = shape
     num_pages, kv_heads, page_size = _check_pages(pages, dim)
     device = pages.device
-    if tokens <= 0 or q.device != device or q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) \
-            or (tokens > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
+    token_stride, head_stride, dim_stride = q.stride()
+    qp = q.data_ptr()
+    if tokens <= 0 or dim_stride != 1 or (heads > 1 and head_stride != dim) or (tokens > 1 and token_stride % 8) or qp % 16 \
+            or q.device != device:
         raise ValueError("q needs contiguous heads, a token stride of a multiple of 8 and 16-byte alignment on the pages' device")
     if heads % kv_heads or heads // kv_heads > 64:
         raise ValueError("heads must be a multiple of kv_heads, at most 64 each")
-    _check_ints(device, table=table, lengths=lengths, starts=starts)
-    if table.ndim != 2 or min(table.shape) <= 0 or lengths.shape != table.shape[:1] or starts.numel() != table.shape[0] + 1:
+    for t in (table, lengths, starts):
+        if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"table, lengths and starts must be contiguous int32 tensors on {device}")
+    if table.ndim != 2 or lengths.shape != table.shape[:1] or starts.numel() != table.shape[0] + 1:
         raise ValueError("Expected table=[requests, width], lengths=[requests], starts=[requests + 1]")
     requests, width = table.shape
-    if requests > MAX_REQUESTS or width * page_size >= 2 ** 31:
-        raise ValueError(f"At most {MAX_REQUESTS} requests and fewer than 2^31 positions")
-    if isinstance(max_new, bool) or not 1 <= max_new <= MAX_NEW:
+    if min(requests, width) <= 0 or requests > MAX_REQUESTS or width * page_size >= 2 ** 31:
+        raise ValueError(f"From 1 to {MAX_REQUESTS} requests and fewer than 2^31 positions")
+    if max_new is True or not 1 <= max_new <= MAX_NEW:
         raise ValueError(f"max_new must be from 1 to {MAX_NEW}")
     if scale is None:
-        scale = 1.0 / math.sqrt(dim)
+        scale = dim ** -0.5
     elif not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
+    _check_device(device, q)
     if out is not None:
-        if out.dtype != q.dtype or out.device != device or out.shape != q.shape or not out.is_contiguous() \
+        if out.dtype is not dtype or out.device != device or out.shape != shape or not out.is_contiguous() \
                 or out.data_ptr() % 16 or out.requires_grad:
             raise ValueError("out must be contiguous, 16-byte aligned, of q's shape, dtype and device")
-        _disjoint((out,), (q, pages, table, lengths, starts))
-    _check_device(device, q)
+        _disjoint(out, q, pages, table, lengths, starts)
+        tensors = (q, pages, table, lengths, starts, out)
+    else:
+        out = torch.empty(tokens, heads, dim, device=device, dtype=dtype)
+        tensors = (q, pages, table, lengths, starts)
     index = ready(device)
-    if out is None:
-        # q may be a slice of a wider row; out is not.
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty((tokens, heads, dim), device=device, dtype=q.dtype)
     # Scratch of this call alone: a captured graph keeps its own, and nothing has to be zero in it.
     need = _scratch_bytes(index, requests, width, page_size, heads, kv_heads, dim, max_new)
     scratch = torch.empty(need, device=device, dtype=torch.uint8)
     launch("klab_kv_attention", index,
-           (q.data_ptr(), q.stride(0) if tokens > 1 else 0, _DT[q.dtype], pages.data_ptr(), table.data_ptr(),
-            lengths.data_ptr(), starts.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, tokens, requests, width,
-            num_pages, page_size, heads, kv_heads, dim, max_new, scale), (q, pages, table, lengths, starts, out))
+           (qp, token_stride if tokens > 1 else 0, _DT[dtype], pages.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+            starts.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, tokens, requests, width, num_pages, page_size, heads,
+            kv_heads, dim, max_new, scale), tensors)
     return out

@@ -136,7 +136,7 @@ constexpr int kAsRows = 16 * kAsWarps;   // rows of a block
 constexpr int kAsTokens = 16;            // tokens of a call's tile
 constexpr int kAsUnit = 128;             // bytes of a row in a unit: two 64-byte steps
 constexpr int kAsAhead = 4;              // steps whose loads are in flight (two 16-byte loads each)
-constexpr int kAsWindow = 48 * 1024;     // x in shared memory
+constexpr int kAsWindow = 96 * 1024;     // x in shared memory
 constexpr int kAsMinShare = 4;           // units of a share at least
 
 // Columns per 64-byte step and 16-byte x pieces (8 columns of a token) per lane and step.
@@ -260,16 +260,19 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
       const int ln = i & 31, piece = (i >> 5) / NB % P, s = (i >> 5) / (NB * P);
       return COLS * (s0 + s) + (KIND == AD_I8 ? 16 * (ln & 3) + 8 * piece : 32 * piece + 8 * (ln & 3));
     };
-    auto fetch = [&](int i) {
+    for (int i = tid; i < pieces; i += kAsThreads) {  // every copy in flight at once; zeros past M and K
       const int token = token0 + (i >> 5) % NB * 8 + ((i & 31) >> 2), col = column(i);
-      return token < p.m && col < p.k
-                 ? __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token) * p.k + col))
-                 : make_uint4(0u, 0u, 0u, 0u);
-    };
-#pragma unroll 4
-    for (int i = tid; i < pieces; i += kAsThreads) {
-      const uint4 v = fetch(i);
-      if constexpr (KIND != AD_BF16) {  // the largest exponent of the token in the window
+      const bool there = token < p.m && col < p.k;
+      const unsigned short* src = there ? p.x + static_cast<long long>(token) * p.k + col : p.x;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(xs) + 16 * i), "l"(src),
+                   "r"(there ? 16 : 0)
+                   : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (KIND != AD_BF16) {
+      // BF16 -> FP16 times 2^(141 - ef), ef the largest exponent of the token in the window, which lands below 2^15
+      for (int i = tid; i < pieces; i += kAsThreads) {  // this thread's own copies
+        const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
         const unsigned u[4] = {v.x, v.y, v.z, v.w};
         unsigned most = 0;
 #pragma unroll
@@ -279,12 +282,9 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
         ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 2));
         if ((tid & 3) == 0) atomicMax(top + (i >> 5) % NB * 8 + ((i & 31) >> 2), ef);
       }
-      reinterpret_cast<uint4*>(xs)[i] = v;
-    }
-    __syncthreads();
-    if constexpr (KIND != AD_BF16) {  // BF16 -> FP16 times 2^(141 - ef): the largest lands below 2^15
+      __syncthreads();
       for (int i = tid; i < pieces; i += kAsThreads) {
-        const uint4 v = reinterpret_cast<uint4*>(xs)[i];
+        const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
         unsigned u[4] = {v.x, v.y, v.z, v.w};
         const int ef = min(max(top[(i >> 5) % NB * 8 + ((i & 31) >> 2)], 15), 254);
         const float by = __int_as_float((268 - ef) << 23);
@@ -295,8 +295,8 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
         }
         reinterpret_cast<uint4*>(xs)[i] = make_uint4(u[0], u[1], u[2], u[3]);
       }
-      __syncthreads();
     }
+    __syncthreads();
     // ---- the window's steps
     float acc[NB][4];
 #pragma unroll
@@ -444,73 +444,76 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
   }
 }
 
-// 128 rows x 4 tokens of the result: one thread per row.
-constexpr int kJoinTokens = 4;
+// 128 rows of one token, a thread per row. The token's adapter and its rows of B are read before the streaming kernel has
+// ended: all its CTAs have then passed their wait for what came before the call.
 template <int KIND>
 __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParams p) {
-  __shared__ float ts[kJoinTokens][kMaxRank];
-  __shared__ int ids[kJoinTokens];
+  __shared__ __align__(16) float ts[kMaxRank];
+  const int tid = threadIdx.x, block = blockIdx.x, row = block * kAsRows + tid, token = blockIdx.y;
+  const int tile = token / kAsTokens, slot = token % kAsTokens;
+  constexpr int kHeld = 8;  // 16-byte runs of B that are asked for ahead
+  const int id = __ldg(p.ids + token);
+  const bool has = id >= 0 && id < p.adapters;
+  const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(has ? id : 0) * p.n + min(row, p.n - 1)) * p.rank);
+  const int runs = has ? p.rank / 8 : 0;
+  uint4 held[kHeld];
+#pragma unroll
+  for (int r = 0; r < kHeld; ++r) held[r] = r < runs ? __ldg(b + r) : make_uint4(0u, 0u, 0u, 0u);
+  const float c = has ? __ldg(p.c + id) : 0.0f;
+  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + min(row, p.n - 1)) : 1.0f;
   grid_dependency_wait();
   grid_launch_dependents();
-  const int tid = threadIdx.x, block = blockIdx.x, row = block * kAsRows + tid;
-  const int tile = blockIdx.y / (kAsTokens / kJoinTokens), first = blockIdx.y % (kAsTokens / kJoinTokens) * kJoinTokens;
-  const int token0 = tile * kAsTokens + first, tokens = min(kJoinTokens, p.m - token0);
-  if (tokens <= 0) return;
-  const int a_total = p.a_blocks * p.a_units;
-  if (tid < tokens) {
-    const int id = __ldg(p.ids + token0 + tid);
-    ids[tid] = id >= 0 && id < p.adapters ? id : -1;
-  }
   // The shares of the block, in order.
-  const int begin = a_total + block * p.w_units;
+  const int begin = p.a_blocks * p.a_units + block * p.w_units;
   const int pieces = (begin + p.w_units - 1) / p.share - begin / p.share + 1;
-  const float* from = p.w_part + ((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces * kAsTokens + first) * kAsRows + tid;
-  float y[kJoinTokens] = {};
-#pragma unroll 4
-  for (int q = 0; q < pieces; ++q)
+  const float* from = p.w_part + ((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces * kAsTokens + slot) * kAsRows + tid;
+  float y = 0.0f;
+  for (int q0 = 0; q0 < pieces; q0 += 8) {
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < kJoinTokens; ++j)
-      if (j < tokens) y[j] += __ldcg(from + (static_cast<long long>(q) * kAsTokens + j) * kAsRows);
-  __syncthreads();
-  for (int i = tid; i < tokens * p.rank; i += kAsRows) {
-    const int j = i / p.rank, r = i - j * p.rank;
-    if (ids[j] < 0) continue;
-    const int group = (first + j) * p.groups + r / 16, ablock = group / kAsWarps;
+    for (int q = 0; q < 8; ++q)
+      v[q] = q0 + q < pieces ? __ldcg(from + static_cast<long long>(q0 + q) * kAsTokens * kAsRows) : 0.0f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) y += v[q];
+  }
+  for (int r = tid; r < 8 * runs; r += kAsRows) {
+    const int group = slot * p.groups + r / 16, ablock = group / kAsWarps;
     const int abegin = ablock * p.a_units, apieces = (abegin + p.a_units - 1) / p.share - abegin / p.share + 1;
     const float* src = p.a_part + (static_cast<long long>(tile) * p.a_blocks + ablock) * p.a_pieces * kAsRows +
                        16 * (group % kAsWarps) + r % 16;
-    float v = 0.0f;
-#pragma unroll 8
-    for (int q = 0; q < apieces; ++q) v += __ldcg(src + static_cast<long long>(q) * kAsRows);
-    ts[j][r] = mul_rn(v, __ldg(p.c + ids[j]));
+    float t = 0.0f;
+    for (int q0 = 0; q0 < apieces; q0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = q0 + q < apieces ? __ldcg(src + static_cast<long long>(q0 + q) * kAsRows) : 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) t += v[q];
+    }
+    ts[r] = mul_rn(t, c);
   }
   __syncthreads();
   if (row >= p.n) return;
-  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + row) : 1.0f;
+  if (KIND == AD_I8) y = mul_rn(y, scale);
+  if (has) {
+    float s0 = 0.0f, s1 = 0.0f;
+    auto dot = [&](uint4 w, int r) {
+      const float4 lo = reinterpret_cast<const float4*>(ts)[2 * r], hi = reinterpret_cast<const float4*>(ts)[2 * r + 1];
+      s0 = fma_rn(lo.x, bf16lo(w.x), s0), s1 = fma_rn(lo.y, bf16hi(w.x), s1);
+      s0 = fma_rn(lo.z, bf16lo(w.y), s0), s1 = fma_rn(lo.w, bf16hi(w.y), s1);
+      s0 = fma_rn(hi.x, bf16lo(w.z), s0), s1 = fma_rn(hi.y, bf16hi(w.z), s1);
+      s0 = fma_rn(hi.z, bf16lo(w.w), s0), s1 = fma_rn(hi.w, bf16hi(w.w), s1);
+    };
 #pragma unroll
-  for (int j = 0; j < kJoinTokens; ++j) {
-    if (j >= tokens) break;
-    float v = KIND == AD_I8 ? mul_rn(y[j], scale) : y[j];
-    if (ids[j] >= 0) {
-      const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(ids[j]) * p.n + row) * p.rank);
-      float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll 8
-      for (int r = 0; r < p.rank / 8; ++r) {
-        const uint4 w = __ldg(b + r);
-        const float* tj = ts[j] + 8 * r;
-        s0 = fma_rn(tj[0], bf16lo(w.x), s0), s1 = fma_rn(tj[1], bf16hi(w.x), s1);
-        s0 = fma_rn(tj[2], bf16lo(w.y), s0), s1 = fma_rn(tj[3], bf16hi(w.y), s1);
-        s0 = fma_rn(tj[4], bf16lo(w.z), s0), s1 = fma_rn(tj[5], bf16hi(w.z), s1);
-        s0 = fma_rn(tj[6], bf16lo(w.w), s0), s1 = fma_rn(tj[7], bf16hi(w.w), s1);
-      }
-      v = add_rn(v, add_rn(s0, s1));
-    }
-    const long long at = static_cast<long long>(token0 + j) * p.ldo + row;
-    if (p.out_f32)
-      static_cast<float*>(p.out)[at] = v;
-    else
-      static_cast<unsigned short*>(p.out)[at] = f32_to_bf16_rn(v);
+    for (int r = 0; r < kHeld; ++r)
+      if (r < runs) dot(held[r], r);
+    for (int r = kHeld; r < runs; ++r) dot(__ldg(b + r), r);
+    y = add_rn(y, add_rn(s0, s1));
   }
+  const long long at = static_cast<long long>(token) * p.ldo + row;
+  if (p.out_f32)
+    static_cast<float*>(p.out)[at] = y;
+  else
+    static_cast<unsigned short*>(p.out)[at] = f32_to_bf16_rn(y);
 }
 
 struct StreamPlan {
@@ -575,7 +578,7 @@ int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t strea
   }
   const int rc = launch_stream(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, kAsWindow, p, stream);
   if (rc) return rc;
-  return launch_stream(adapter_join_kernel<KIND>, dim3(p.w_blocks, plan.tiles * (kAsTokens / kJoinTokens)), kAsRows, 0, p,
+  return launch_stream(adapter_join_kernel<KIND>, dim3(p.w_blocks, p.m), kAsRows, 0, p,
                        stream);
 }
 
@@ -652,7 +655,7 @@ KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const v
     const int rc = sm_count(&sms);
     if (rc) return rc;
     const StreamPlan plan = plan_stream(kind, q, 2 * sms);
-    if ((reinterpret_cast<uintptr_t>(w) & 15) == 0 && q.row_bytes % 16 == 0 && plan.tiles * (kAsTokens / kJoinTokens) <= 65535 &&
+    if ((reinterpret_cast<uintptr_t>(w) & 15) == 0 && q.row_bytes % 16 == 0 &&
         static_cast<long long>(q.a_blocks) * q.a_units + static_cast<long long>(q.w_blocks) * q.w_units < INT_MAX) {
       if (kind != AD_BF16 && !aux) return KLAB_E_INVALID;
       if (kind == AD_FP4 && k % 32) return KLAB_E_SHAPE;

@@ -121,26 +121,26 @@ struct Place {
   long long block;
 };
 
+template <int D>
 __device__ __forceinline__ Place place_of(const RowParams& p, unsigned at) {
   Place w;
-  const unsigned runs = p.dim / 8;  // a power of two
-  const int shift = 31 - __clz(static_cast<int>(runs));
-  w.c = at & (runs - 1);
-  const unsigned rest = at >> (shift + 1), pair = rest / p.kv_heads;
+  constexpr unsigned kRuns = D / 8;
+  w.c = at % kRuns;
+  const unsigned rest = at / (2 * kRuns), pair = rest / p.kv_heads;
   w.head = rest - pair * p.kv_heads;
-  w.token = 2 * pair + (at >> shift & 1);
+  w.token = 2 * pair + at / kRuns % 2;
   w.slot = w.token < p.tokens ? p.slots[w.token] : -1;
-  w.block = kv_block_offset(w.slot, w.head, p.num_pages, p.kv_heads, p.page_shift, p.dim);
+  w.block = kv_block_offset(w.slot, w.head, p.num_pages, p.kv_heads, p.page_shift, D);
   if (w.slot != -1 && w.block < 0) record_status(p.status, kStatusBadPage);
   return w;
 }
 
-template <bool kBf16>
+template <bool kBf16, int D>
 __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const RowParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const unsigned at = blockIdx.x * kStoreThreads + threadIdx.x;
-  const Place w = place_of(p, at);  // a thread past the end has a slot of -1 and stays for the shuffles
+  const Place w = place_of<D>(p, at);  // a thread past the end has a slot of -1 and stays for the shuffles
   uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
   if (w.block >= 0) {
     const long long row = w.token;
@@ -159,26 +159,26 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const RowParams
   unsigned short k_scale, v_scale;
   const unsigned k_codes = quantize8<kBf16>(k, k_scale), v_codes = quantize8<kBf16>(v, v_scale);
   // The other token of the pair: its V codes and slot (heads of 256 take a warp each and write halves).
-  const int other = p.dim / 8;
+  constexpr int other = D / 8;
   const unsigned v_other = __shfl_xor_sync(0xffffffffu, v_codes, other & 31);
   const int slot_other = __shfl_xor_sync(0xffffffffu, w.slot, other & 31);
   if (w.block < 0) return;
   unsigned short* to = p.pages + w.block / 2;
   const int r = w.slot & (kKvBlock - 1);
-  *reinterpret_cast<unsigned*>(to + kv_k_piece(r, 2 * w.c, p.dim)) = k_codes;
+  *reinterpret_cast<unsigned*>(to + kv_k_piece(r, 2 * w.c, D)) = k_codes;
   // Pieces 2 c and 2 c + 1 (dims 8 c .. + 3, 8 c + 4 .. + 7): neighbouring g of one group.
   if (other < 32 && slot_other == (w.slot ^ 1)) {
     if ((w.slot & 1) == 0)
-      *reinterpret_cast<unsigned*>(to + kv_v_piece(r, 2 * w.c, p.dim)) = __byte_perm(v_codes, v_other, 0x5410);
+      *reinterpret_cast<unsigned*>(to + kv_v_piece(r, 2 * w.c, D)) = __byte_perm(v_codes, v_other, 0x5410);
     else
-      *reinterpret_cast<unsigned*>(to + kv_v_piece(r & ~1, 2 * w.c + 1, p.dim)) = __byte_perm(v_other, v_codes, 0x7632);
+      *reinterpret_cast<unsigned*>(to + kv_v_piece(r & ~1, 2 * w.c + 1, D)) = __byte_perm(v_other, v_codes, 0x7632);
   } else {
-    to[kv_v_piece(r, 2 * w.c, p.dim)] = static_cast<unsigned short>(v_codes);
-    to[kv_v_piece(r, 2 * w.c + 1, p.dim)] = static_cast<unsigned short>(v_codes >> 16);
+    to[kv_v_piece(r, 2 * w.c, D)] = static_cast<unsigned short>(v_codes);
+    to[kv_v_piece(r, 2 * w.c + 1, D)] = static_cast<unsigned short>(v_codes >> 16);
   }
   if ((w.c & 3) == 0) {
-    to[kv_k_scale(r, w.c >> 2, p.dim)] = k_scale;
-    to[kv_v_scale(r, w.c >> 2, p.dim)] = v_scale;
+    to[kv_k_scale(r, w.c >> 2, D)] = k_scale;
+    to[kv_v_scale(r, w.c >> 2, D)] = v_scale;
   }
 }
 
@@ -209,24 +209,24 @@ __device__ __forceinline__ void put8(void* out, long long at, unsigned codes, fl
   }
 }
 
-template <int kOut>
+template <int kOut, int D>
 __global__ void __launch_bounds__(kStoreThreads) kv_read_kernel(const RowParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const unsigned at = blockIdx.x * kStoreThreads + threadIdx.x;
-  const Place w = place_of(p, at);
+  const Place w = place_of<D>(p, at);
   if (w.token >= p.tokens) return;
   unsigned k_codes = 0x88888888u, v_codes = 0x88888888u;
   float k_scale = 0.0f, v_scale = 0.0f;
   if (w.block >= 0) {
     const unsigned short* from = p.pages + w.block / 2;
     const int r = w.slot & (kKvBlock - 1);
-    k_codes = *reinterpret_cast<const unsigned*>(from + kv_k_piece(r, 2 * w.c, p.dim));
-    v_codes = from[kv_v_piece(r, 2 * w.c, p.dim)] | static_cast<unsigned>(from[kv_v_piece(r, 2 * w.c + 1, p.dim)]) << 16;
-    k_scale = f16_to_f32(from[kv_k_scale(r, w.c >> 2, p.dim)]);
-    v_scale = f16_to_f32(from[kv_v_scale(r, w.c >> 2, p.dim)]);
+    k_codes = *reinterpret_cast<const unsigned*>(from + kv_k_piece(r, 2 * w.c, D));
+    v_codes = from[kv_v_piece(r, 2 * w.c, D)] | static_cast<unsigned>(from[kv_v_piece(r, 2 * w.c + 1, D)]) << 16;
+    k_scale = f16_to_f32(from[kv_k_scale(r, w.c >> 2, D)]);
+    v_scale = f16_to_f32(from[kv_v_scale(r, w.c >> 2, D)]);
   }
-  const long long to = (static_cast<long long>(w.token) * p.kv_heads + w.head) * (p.dim / 8) + w.c;
+  const long long to = (static_cast<long long>(w.token) * p.kv_heads + w.head) * (D / 8) + w.c;
   put8<kOut>(p.k_out, to, k_codes, k_scale);
   put8<kOut>(p.v_out, to, v_codes, v_scale);
 }
@@ -253,6 +253,15 @@ int launch_rows(Kernel kernel, const RowParams& p, void* stream) {
   cfg.attrs = attr;
   cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int kOut>
+int launch_read(const RowParams& p, void* stream) {
+  switch (p.dim) {
+    case 64: return launch_rows(kv_read_kernel<kOut, 64>, p, stream);
+    case 128: return launch_rows(kv_read_kernel<kOut, 128>, p, stream);
+    default: return launch_rows(kv_read_kernel<kOut, 256>, p, stream);
+  }
 }
 
 }  // namespace
@@ -296,8 +305,12 @@ KLAB_API int klab_kv_store(const void* k, const void* v, int dtype, long long k_
   p.kv_heads = kv_heads;
   p.dim = dim;
   p.page_shift = kv_page_shift(page_size);
-  return dtype == KLAB_DT_BF16 ? launch_rows(kv_store_kernel<true>, p, stream)
-                               : launch_rows(kv_store_kernel<false>, p, stream);
+  const bool bf16 = dtype == KLAB_DT_BF16;
+  switch (dim) {
+    case 64: return bf16 ? launch_rows(kv_store_kernel<true, 64>, p, stream) : launch_rows(kv_store_kernel<false, 64>, p, stream);
+    case 128: return bf16 ? launch_rows(kv_store_kernel<true, 128>, p, stream) : launch_rows(kv_store_kernel<false, 128>, p, stream);
+    default: return bf16 ? launch_rows(kv_store_kernel<true, 256>, p, stream) : launch_rows(kv_store_kernel<false, 256>, p, stream);
+  }
 }
 
 KLAB_API int klab_kv_read(const void* pages, const int* slots, void* k_out, void* v_out, int dtype, int tokens,
@@ -320,9 +333,9 @@ KLAB_API int klab_kv_read(const void* pages, const int* slots, void* k_out, void
   p.dim = dim;
   p.page_shift = kv_page_shift(page_size);
   switch (dtype) {
-    case KLAB_DT_BF16: return launch_rows(kv_read_kernel<KLAB_DT_BF16>, p, stream);
-    case KLAB_DT_F16: return launch_rows(kv_read_kernel<KLAB_DT_F16>, p, stream);
-    case KLAB_DT_F32: return launch_rows(kv_read_kernel<KLAB_DT_F32>, p, stream);
+    case KLAB_DT_BF16: return launch_read<KLAB_DT_BF16>(p, stream);
+    case KLAB_DT_F16: return launch_read<KLAB_DT_F16>(p, stream);
+    case KLAB_DT_F32: return launch_read<KLAB_DT_F32>(p, stream);
     default: return KLAB_E_UNSUPPORTED;
   }
 }

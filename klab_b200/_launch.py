@@ -1,12 +1,18 @@
-"""Launch path of the batched operators: torch's current stream of a device, the native call, and the caching allocator's
-stream bookkeeping (_native.record) with as little host time as the calls themselves allow.
+"""Launch path of the batched operators.
 
-A decode step makes several of these calls per layer, so their host time is the step's time when the batch is small: the
-stream comes as a raw handle, the device is switched only when it is not the current one, and Stream objects are kept
-per handle for record_stream.
+A decode step makes several of these calls per layer, so their host time is the step's time when the batch is small. Plain
+calls go through the CPython module built from csrc/torch_binding.cpp (`fast`, loaded with the first device), which checks,
+allocates and launches in a few microseconds; whatever it answers None to comes back to the Python wrappers, which raise or
+launch through ctypes (`launch`): torch's current stream, the device switched only when it is not the current one, and the
+caching allocator told which stream used the tensors (_native.record).
 """
 
 from __future__ import annotations
+
+import ctypes as ct
+import importlib.machinery
+import importlib.util
+import threading
 
 import torch
 
@@ -19,6 +25,24 @@ _capturing = torch._C._cuda_isCurrentStreamCapturing
 _functions = {}
 _streams = {}
 _ready = set()
+_lock = threading.Lock()
+# The entry points in the order that the binding takes them.
+_ENTRIES = ("klab_kv_build_step", "klab_kv_store", "klab_kv_read", "klab_kv_attention", "klab_kv_attention_scratch",
+            "klab_adapter_linear", "klab_adapter_scratch")
+BINDING = _native.LIB_DIR / "klab_torch.so"
+fast = None  # the binding, once a device is ready
+
+
+def load_binding():
+    """The binding module with _native's entry points (no device needed)."""
+    if not BINDING.exists():
+        raise RuntimeError(f"{BINDING} is missing: build it with `python -m klab_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("klab_torch", str(BINDING))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("klab_torch", loader))
+    loader.exec_module(module)
+    lib = _native.lib()
+    module.bind(*(ct.cast(getattr(lib, name), ct.c_void_p).value for name in _ENTRIES))
+    return module
 
 
 def ready(device):
@@ -28,7 +52,13 @@ def ready(device):
         if device.type != "cuda":
             raise ValueError("Expected CUDA tensors")
         get_module(device)
-        _ready.add(index)
+        global fast
+        with _lock:
+            module = fast or load_binding()
+            if index < 64:
+                module.mark_ready(index)
+            fast = module
+            _ready.add(index)
     return index
 
 

@@ -15,7 +15,7 @@ from functools import lru_cache
 
 import torch
 
-from . import _native
+from . import _launch, _native
 from ._launch import launch, ready
 from .compressed_bf16 import PackedBF16
 from .fp4 import FP4F16Weights
@@ -79,6 +79,18 @@ def adapter_linear(x, w, a, b, scales, ids, *, out=None, output_dtype=torch.bflo
     [adapters, N, rank] (rank a multiple of 8, at most 256), scales FP32 [adapters], ids int32 [M]. Returns [M, N] in
     output_dtype (BF16 or FP32). K must be a multiple of 8. An index outside -1 .. adapters - 1 counts as -1 and sets the
     device status to 6."""
+    if _launch.fast is not None and output_dtype in (torch.bfloat16, torch.float32):
+        fp32 = output_dtype is torch.float32
+        if type(w) is torch.Tensor:
+            done = _launch.fast.adapter_linear(_native.W_BF16, x, w, None, a, b, scales, ids, out, fp32)
+        elif type(w) is Int8Weights:
+            done = _launch.fast.adapter_linear(_native.W_I8_ROW, x, w.codes, w.scales, a, b, scales, ids, out, fp32)
+        elif type(w) is FP4F16Weights:
+            done = _launch.fast.adapter_linear(_native.W_FP4_G32H, x, w.packed, w.scales, a, b, scales, ids, out, fp32)
+        else:
+            done = None
+        if done is not None:
+            return done if type(done) is not int else _native.check(done, "klab_adapter_linear")
     if x.ndim != 2 or x.dtype != torch.bfloat16:
         raise ValueError("Expected BF16 x [M,K]")
     m, k = x.shape

@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -26,6 +27,7 @@ OBJ = OUT / "obj"
 LIBRARY = OUT / "libklab_b200.so"
 ALIAS = OUT / "libkernel_lab.so"  # the reference's library name (native/build/libkernel_lab.so)
 PREFETCH_CUBIN = OUT / "prefetch_kernels.cubin"
+BINDING = OUT / "klab_torch.so"           # CPython module over torch (csrc/torch_binding.cpp)
 LAUNCHER = HERE.parent / "bin" / "klab"   # the reference's bin/klab (native/cli.cpp)
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -108,8 +110,31 @@ def build(clean: bool = False, verbose: bool = False, out_dir: Path | None = Non
         ALIAS.unlink()
     ALIAS.symlink_to(LIBRARY.name)
     if out_dir is None:
+        build_binding()
         build_launcher()
     return LIBRARY
+
+
+def build_binding() -> Path:
+    """klab_torch.so from csrc/torch_binding.cpp (g++, torch's headers); rebuilt when torch's version changes."""
+    import torch
+
+    source, stamp = CSRC / "torch_binding.cpp", OBJ / "klab_torch.version"
+    version = f"{torch.__version__} {sys.version}"
+    if _stale(BINDING, [source, *_headers()]) or not stamp.exists() or stamp.read_text() != version:
+        root = Path(torch.__file__).resolve().parent
+        cuda = Path(nvcc()).resolve().parents[1]
+        cxx = shutil.which(os.environ.get("CXX", "g++")) or "g++"
+        tmp = BINDING.with_suffix(".new")
+        includes = [INCLUDE, root / "include", root / "include/torch/csrc/api/include", cuda / "include",
+                    sysconfig.get_paths()["include"]]
+        _run([cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{i}" for i in includes],
+              str(source), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+              "-ltorch", "-ltorch_python"])
+        tmp.replace(BINDING)
+        stamp.write_text(version)
+    return BINDING
 
 
 def build_launcher() -> Path:

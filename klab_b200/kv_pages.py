@@ -25,7 +25,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _native
+from . import _launch, _native
 from ._launch import launch, ready
 
 HEAD_DIMS = (64, 128, 256)
@@ -133,6 +133,10 @@ def build_step(new_tokens, lengths, table, free_pages, free_count, *, page_size,
     themselves, for a captured step). max_tokens bounds the step's tokens. All or nothing: where result is not STEP_OK,
     no page was given out and there are no tokens.
     """
+    if _launch.fast is not None:
+        step = _launch.fast.build_step(new_tokens, lengths, table, free_pages, free_count, page_size, max_tokens, inplace)
+        if step is not None:
+            return BatchStep(*step) if type(step) is tuple else _native.check(step, "klab_kv_build_step")
     requests, width, num_pages = _check_state(lengths, table, free_pages, free_count, page_size)
     device = lengths.device
     _check_ints(device, new_tokens=new_tokens)
@@ -206,6 +210,10 @@ def store(k, v, pages, slots) -> None:
     """Rows k, v [tokens, kv_heads, head_dim] (BF16 or FP16; any token and head strides that are multiples of 4 elements,
     such as slices of a fused projection's output) into pages at slots [tokens] (int32). A slot of -1 is skipped; two
     tokens of one call must not name the same slot."""
+    if _launch.fast is not None:
+        done = _launch.fast.store(k, v, pages, slots)
+        if done is not None:
+            return None if done is True else _native.check(done, "klab_kv_store")
     shape, dtype = k.shape, k.dtype
     if len(shape) != 3 or v.shape != shape or dtype not in _DT or v.dtype is not dtype:
         raise ValueError("Expected k and v [tokens, kv_heads, head_dim] in BF16 or FP16")
@@ -236,6 +244,10 @@ def store(k, v, pages, slots) -> None:
 def read(pages, slots, head_dim, dtype=torch.bfloat16):
     """(k, v) [tokens, kv_heads, head_dim] as held at slots [tokens]: (code - 8) * scale, rounded once to dtype (float32:
     exact). Zeros for a slot of -1."""
+    if _launch.fast is not None:
+        rows = _launch.fast.read(pages, slots, head_dim, _ODT.get(dtype))
+        if rows is not None:
+            return rows if type(rows) is tuple else _native.check(rows, "klab_kv_read")
     num_pages, kv_heads, page_size = _check_pages(pages, head_dim)
     device = pages.device
     if dtype not in _ODT or slots.ndim != 1 or slots.numel() <= 0:
@@ -273,6 +285,10 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
     below lengths[i] - n + j + 1, and a row that sees none gives zeros. scale defaults to 1 / sqrt(head_dim). Rows of q
     that belong to no request leave their rows of `out` as they were.
     """
+    if _launch.fast is not None:
+        done = _launch.fast.attention(q, pages, table, lengths, starts, max_new, scale, out)
+        if done is not None:
+            return done if type(done) is not int else _native.check(done, "klab_kv_attention")
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or dtype not in _DT:
         raise ValueError("Expected q [tokens, heads, head_dim] in BF16 or FP16")

@@ -464,3 +464,68 @@ def test_two_graphs_and_another_stream_share_nothing():
     torch.cuda.synchronize()
     for got, w in zip((*outs, other), want):
         assert torch.equal(got, w)
+
+
+def test_both_launch_paths_agree(monkeypatch):
+    """The binding serves plain calls; without it the wrappers launch the same kernels through ctypes."""
+    from klab_b200 import _launch, kv_pages
+
+    def everything():
+        q, buf, table, ln, st, starts, k, v = attention_case([300, 40], [1, 2], 8, 2, 64, 16, "bf16", 6)
+        out = torch.zeros(q.shape, device="cuda", dtype=q.dtype)
+        assert kv_pages.attention(q, buf, table, ln, st, max_new=2, out=out) is out
+        rows = kv_pages.read(buf, i32([5, -1, 33]), 64, dtype=torch.float16)
+        step = kv_pages.build_step(i32([3, 0]), ln, table, i32(np.arange(40)), i32([5]), page_size=16, max_tokens=8)
+        count, lengths = i32([5]), ln.clone()
+        moved = kv_pages.build_step(i32([1, 1]), lengths, table, i32(np.arange(40)), count, page_size=16, max_tokens=8, inplace=True)
+        assert moved.lengths is lengths and moved.free_count is count
+        return (out, kv_pages.attention(q, buf, table, ln, st, max_new=2, scale=0.3), *rows, *step, *moved)
+
+    everything()
+    assert _launch.fast is not None
+    served = []
+    with monkeypatch.context() as m:
+        class Counting:
+            def __getattr__(self, name):
+                def call(*a):
+                    r = getattr(real, name)(*a)
+                    served.append(r is not None)
+                    return r
+                return call
+        real = _launch.fast
+        m.setattr(_launch, "fast", Counting())
+        first = everything()
+    assert served and all(served)
+    monkeypatch.setattr(_launch, "fast", None)
+    for a, b in zip(first, everything()):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_refusals_on_the_gpu():
+    """What the binding does not serve is refused by the wrappers, with a device ready."""
+    from klab_b200 import kv_pages
+
+    q, buf, table, ln, st, starts, k, v = attention_case([30, 4], [1, 1], 8, 2, 64, 16, "bf16", 6)
+    for bad in ({"max_new": 0}, {"max_new": 17}, {"scale": -1.0}, {"scale": float("inf")}, {"out": q}, {"lengths": ln.long()},
+                {"lengths": ln.cpu()}, {"starts": st[:2]}, {"q": q.float()}, {"q": q[:, :7]}, {"pages": buf[:, :, :-16]},
+                {"pages": buf.cpu()}, {"table": table.t()}, {"q": q.clone().requires_grad_()}):
+        a = {"q": q, "pages": buf, "table": table, "lengths": ln, "starts": st, **bad}
+        with pytest.raises(ValueError):
+            kv_pages.attention(**a)
+    slots = i32(np.arange(34))
+    for bad in ((k, v.half(), buf, slots), (k, v, buf, slots[:3]), (k, v, buf, slots.long()), (k[:, :1], v[:, :1], buf, slots),
+                (k.cpu(), v, buf, slots)):
+        with pytest.raises(ValueError):
+            kv_pages.store(*bad)
+    for bad in ((buf, slots, 96), (buf, slots.long(), 64), (buf, slots, 128)):
+        with pytest.raises(ValueError):
+            kv_pages.read(*bad)
+    with pytest.raises(ValueError):
+        kv_pages.read(buf, slots, 64, dtype=torch.float64)
+    free, count = i32([0] * 9), i32([3])
+    for bad in ({"page_size": 24}, {"max_tokens": 0}, {"new_tokens": i32([1])}, {"lengths": table[:, 0]}, {"free_count": free},
+                {"lengths": table.view(-1)[:2]}):
+        a = {"new_tokens": i32([1, 1]), "lengths": ln, "table": table, "free_pages": free, "free_count": count,
+             "page_size": 16, "max_tokens": 4, **bad}
+        with pytest.raises(ValueError):
+            kv_pages.build_step(**a)

@@ -185,3 +185,28 @@ def test_attention_arguments():
         kv_pages.attention(**good)
     with pytest.raises(ValueError, match="requires_grad"):
         kv_pages.attention(**{**good, "q": q.clone().requires_grad_()})
+
+
+def test_binding_leaves_what_it_does_not_serve_to_the_wrappers():
+    """Without a ready device every call comes back None (the wrapper's checks then decide); its own setup is checked."""
+    from klab_b200 import _launch
+
+    module = _launch.load_binding()
+    pages = kv_pages.empty_pages(4, 2, 16, 128, device="cpu")
+    k, slots = torch.zeros(3, 2, 128, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    t = tables()
+    assert module.store(k, k, pages, slots) is None and module.store(k, k) is None and module.store(1, k, pages, None) is None
+    assert module.read(pages, slots, 128, 0) is None and module.read(pages, slots, 128, None) is None
+    q, starts = torch.zeros(3, 8, 128, dtype=torch.bfloat16), torch.arange(4, dtype=torch.int32)
+    for scale, out in ((None, None), (0.5, q), (-1.0, None), ("x", None), (None, 3)):
+        assert module.attention(q, pages, t["table"], t["lengths"], starts, 1, scale, out) is None
+    assert module.build_step(t["lengths"], *t.values(), 16, 9, False) is None
+    assert module.build_step(t["lengths"], *t.values(), 16.0, 9, None) is None
+    x, a = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(3, 8, 64, dtype=torch.bfloat16)
+    assert module.adapter_linear(0, x, x, None, a, a, t["lengths"], slots, None, False) is None
+    with pytest.raises(ValueError):
+        module.bind(0, 0, 0, 0, 0, 0, 0)
+    with pytest.raises(ValueError):
+        module.bind(1)
+    with pytest.raises(ValueError):
+        module.mark_ready(64)

@@ -180,29 +180,28 @@ struct Share {
 };
 
 __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int ctas, bool report) {
-  constexpr int kEach = 4;  // requests per lane and pass
+  constexpr int kEach = 4;  // chunks of 32 requests whose loads are in flight at once
   const int lane = threadIdx.x & 31;
-  Request r[kEach];
   bool bad = false;
   auto load = [&](int base) {
-    int length[kEach] = {}, start[kEach] = {}, end[kEach] = {};
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int i = base + 32 * j + lane;
-      if (base + 32 * j < p.requests && i < p.requests) {
-        length[j] = __ldg(p.lengths + i);
-        start[j] = __ldg(p.starts + i);
-        end[j] = __ldg(p.starts + i + 1);
-      }
+    const int i = base + lane;
+    int length = 0, start = 0, end = 0;
+    if (i < p.requests) {
+      length = __ldg(p.lengths + i);
+      start = __ldg(p.starts + i);
+      end = __ldg(p.starts + i + 1);
     }
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) r[j] = make_request(p, length[j], start[j], end[j], bad);
+    return make_request(p, length, start, end, bad);
   };
-  int all = 0;
-  for (int base = 0; base < p.requests; base += 32 * kEach) {
-    load(base);
+  Request r = load(0);  // lane's request of a chunk
+  int all = r.tiles * r.units;
+  for (int base = 32; base < p.requests; base += 32 * kEach) {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) all += r[j].tiles * r[j].units;
+    for (int j = 0; j < kEach; ++j)
+      if (base + 32 * j < p.requests) {
+        const Request q = load(base + 32 * j);
+        all += q.tiles * q.units;
+      }
   }
   all = __reduce_add_sync(0xffffffffu, all);
   if (bad && report) record_status(p.status, kStatusBadLength);
@@ -210,41 +209,36 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
   it.share = max(p.whole ? 1 : kMinShare, (all + ctas - 1) / ctas);
   it.pos = min(static_cast<long long>(cta) * it.share, static_cast<long long>(all));
   it.end = min(it.pos + it.share, all);
-  it.request = it.tile = it.unit = it.r.tiles = 0;
+  it.request = it.tile = it.unit = 0;
   if (it.pos >= it.end) return it;
-  int carry = 0;
-  for (int base = 0; base < p.requests; base += 32 * kEach) {
-    if (p.requests > 32 * kEach) load(base);
+  int left = it.pos;  // units from the start of the chunk
+  for (int base = 0;; r = load(base += 32)) {
+    const int mine = r.tiles * r.units;
+    int upto = mine;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      if (base + 32 * j < p.requests && it.r.tiles == 0) {
-        const int mine = r[j].tiles * r[j].units;
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, upto, d);
-          if (lane >= d) upto += up;
-        }
-        const int at = it.pos - carry - (upto - mine);
-        const unsigned owner = __ballot_sync(0xffffffffu, at >= 0 && at < mine);
-        if (owner) {
-          const int from = __ffs(owner) - 1;
-          it.request = base + 32 * j + from;
-          it.r.length = __shfl_sync(0xffffffffu, r[j].length, from);
-          it.r.fresh = __shfl_sync(0xffffffffu, r[j].fresh, from);
-          it.r.token0 = __shfl_sync(0xffffffffu, r[j].token0, from);
-          it.r.tiles = __shfl_sync(0xffffffffu, r[j].tiles, from);
-          it.r.units = __shfl_sync(0xffffffffu, r[j].units, from);
-          const int in_request = __shfl_sync(0xffffffffu, at, from);
-          it.tile = in_request / it.r.units;
-          it.unit = in_request - it.tile * it.r.units;
-        }
-        carry += __shfl_sync(0xffffffffu, upto, 31);
-      }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += up;
     }
-    if (it.r.tiles) break;
+    const int before = upto - mine;
+    const unsigned owner = __ballot_sync(0xffffffffu, left >= before && left < upto);
+    if (owner) {
+      const int from = __ffs(owner) - 1;
+      it.request = base + from;
+      it.r.length = __shfl_sync(0xffffffffu, r.length, from);
+      it.r.fresh = __shfl_sync(0xffffffffu, r.fresh, from);
+      it.r.token0 = __shfl_sync(0xffffffffu, r.token0, from);
+      it.r.tiles = __shfl_sync(0xffffffffu, r.tiles, from);
+      it.r.units = __shfl_sync(0xffffffffu, r.units, from);
+      it.unit = left - __shfl_sync(0xffffffffu, before, from);
+      if (it.r.tiles > 1) {
+        it.tile = it.unit / it.r.units;
+        it.unit -= it.tile * it.r.units;
+      }
+      return it;
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  return it;
 }
 
 // The segment behind this one (there is one while pos < end).
@@ -723,7 +717,7 @@ __global__ void __launch_bounds__(kThreads) kv_combine_kernel(const KvAttnParams
   grid_launch_dependents();
   const Header h = p.headers[blockIdx.x];
   if (h.last < 0) return;
-  const int kvh = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kvh = blockIdx.y, tid = threadIdx.x;
   constexpr int kCols = D / 4;
   const int parts = h.last - h.first, records = parts + 1, mine = blockIdx.x - h.first - 1;
   const int total = h.rows * kCols, share = (total + parts - 1) / parts;

@@ -4,19 +4,21 @@
 //
 // BF16, INT8 per-row and E2M1/FP16-per-32 weights with 16-byte rows: two launches.
 //   adapter_stream_kernel reads W and the tokens' A once, as one list of work: a block is 128 rows (8 warps x 16 rows) of W,
-//   or 8 groups of 16 rows of the tokens' A (token m's adapter against x, of which column m counts), and a unit is 128
-//   bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM, so any N and K and
-//   any number of adapters keep every SM reading to the end. A warp multiplies its 16 rows by up to 16 tokens on
-//   mma.m16n8k16 with FP32 sums: lane (g, t) loads 16 bytes of rows g and g + 8 straight into the A fragments (the k slots
-//   of an MMA may be any columns as long as x's are the same), eight loads ahead; x lies in shared memory in fragment
-//   order. BF16 weights meet BF16 x; INT8 codes and E2M1 values are exact in FP16 and meet x in FP16 times a power of two
-//   of the (token, window), E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block goes to
-//   scratch in FP32.
+//   or 8 groups of 16 rows of the tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or
+//   256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM, so any N and K
+//   and any number of adapters keep every SM reading to the end. A warp copies its units into a ring of its own (cp.async,
+//   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this takes 31.3) and
+//   multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16 bytes of rows g and
+//   g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies in shared memory in
+//   fragment order. BF16 weights meet BF16 x; INT8 codes and E2M1 values are exact in FP16 and meet x in FP16 times a power
+//   of two of the (token, window), E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block
+//   goes to scratch in FP32.
 //   adapter_join_kernel adds the shares of each block in order, forms t = c (x A^T) the same way, and writes
 //   y + t . B_a[n] with one rounding.
 // Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
 //
-// What bounds it: HBM, the bytes of W and of the distinct adapters.
+// What bounds it: HBM while the units stream (142 MB in 21 us at M = 16, 14336 -> 4096, rank 64), around it launch, the
+// staging of x (1 to 2.5 us) and the join (3 us).
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -134,10 +136,19 @@ constexpr int kAsWarps = 8;
 constexpr int kAsThreads = 32 * kAsWarps;
 constexpr int kAsRows = 16 * kAsWarps;   // rows of a block
 constexpr int kAsTokens = 16;            // tokens of a call's tile
-constexpr int kAsUnit = 128;             // bytes of a row in a unit: two 64-byte steps
-constexpr int kAsAhead = 4;              // steps whose loads are in flight (two 16-byte loads each)
-constexpr int kAsWindow = 96 * 1024;     // x in shared memory
-constexpr int kAsMinShare = 4;           // units of a share at least
+constexpr int kAsWindow = 32 * 1024;     // x in shared memory
+constexpr int kAsMinShare = 2;           // units of a share: fewer would only add records to join
+
+// Bytes of a row in a unit and units of a warp in flight, by the kind of W. Longer runs of a row are better for HBM, shorter
+// units even out short shares: M = 16, 14336 -> 4096 BF16 takes 31.3 us with 256-byte units and 33.4 with 128; M = 8,
+// 4096 -> 14336 INT8 (half the bytes) 17.6 and 16.6.
+__host__ __device__ constexpr int as_unit(int kind) { return kind == AD_BF16 ? 256 : 128; }
+__host__ __device__ constexpr int as_depth(int kind) { return kind == AD_BF16 ? 2 : 3; }
+
+// A warp's ring in shared memory: units of 16 rows, 16-byte chunk c of row r at chunk c ^ 4 (r mod 2), so that the fragment
+// loads (rows g, four chunks each) meet no bank twice.
+__host__ __device__ constexpr int as_slot(int kind) { return 16 * as_unit(kind); }
+__host__ __device__ constexpr int as_smem(int kind) { return kAsWindow + kAsWarps * as_depth(kind) * as_slot(kind); }
 
 // Columns per 64-byte step and 16-byte x pieces (8 columns of a token) per lane and step.
 __host__ __device__ constexpr int as_cols(int kind) { return kind == AD_BF16 ? 32 : kind == AD_I8 ? 64 : 128; }
@@ -202,87 +213,119 @@ __device__ __forceinline__ void transpose_quad(uint4& v, int t) {
     v.z = s0, v.w = s1;
 }
 
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // One piece of a share: units [u0, u1) of a block of kind KIND, for this warp's 16 rows at `base` (nullptr: no rows), of
-// which `rows` exist. Sums of row g (+ 8) and tokens 2 t (+ 1) of each 8-token block end in `sum`.
-template <int KIND, int NB>
+// which `rows` exist; `ring` is the warp's ring. Sums of row g (+ 8) and tokens 2 t (+ 1) of each
+// 8-token block end in `sum`.
+template <int KIND, int NB, int UNIT, int DEPTH>
 __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsigned char* base, long long row_bytes,
                                              const unsigned short* scales, int rows, int u0, int u1, int token0,
-                                             unsigned char* xs, int* top, float (&sum)[NB][4], bool first) {
+                                             unsigned char* xs, unsigned ring, int* top, float (&sum)[NB][4], bool first) {
   constexpr int P = as_pieces(KIND), COLS = as_cols(KIND);
-  constexpr int kStepBytes = P * NB * 512;               // x of one step
-  constexpr int kSteps = kAsWindow / kStepBytes / kAsAhead * kAsAhead;  // steps of a window
+  constexpr int kUnitSteps = UNIT / 64, kSlot = 16 * UNIT;  // an MMA step takes 64 bytes of each row
+  constexpr int kStepBytes = P * NB * 512;  // x of one step
+  constexpr int kSteps = kAsWindow / kStepBytes / kUnitSteps * kUnitSteps;  // steps of a window
   const int tid = threadIdx.x, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int s_end = 2 * u1;
   const bool has0 = base && g < rows, has1 = base && g + 8 < rows;
-  const unsigned char* r0 = base + g * row_bytes + 16 * t;
-  const unsigned char* r1 = r0 + 8 * row_bytes;
-  const long long srow = p.k / 32;  // E2M1: scales of a row, four to a step
-  const bool scales_vec = (srow & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0;
-  uint4 w0[kAsAhead], w1[kAsAhead];
-  uint2 f0[KIND == AD_FP4 ? kAsAhead : 1], f1[KIND == AD_FP4 ? kAsAhead : 1];
-  auto load = [&](int s, int j) {
-    const long long at = 64ll * s;
-    const bool in = s < s_end && at + 16 * t < row_bytes;
-    w0[j] = in && has0 ? ldg128_stream(r0 + at) : make_uint4(0u, 0u, 0u, 0u);
-    w1[j] = in && has1 ? ldg128_stream(r1 + at) : make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (KIND == AD_FP4) {
-      if (scales_vec) {
-        const bool there = s < s_end && 4 * s < srow;
-        f0[j] = there && has0 ? __ldg(reinterpret_cast<const uint2*>(scales + g * srow + 4 * s)) : make_uint2(0u, 0u);
-        f1[j] = there && has1 ? __ldg(reinterpret_cast<const uint2*>(scales + (g + 8) * srow + 4 * s)) : make_uint2(0u, 0u);
-      } else {
-        unsigned short v[8] = {};
+  // Copies go by rows: kRun lanes take a row's bytes of the unit, so HBM sees whole runs of sectors.
+  constexpr int kRun = UNIT / 16, kRowsAtOnce = 32 / kRun;
+  const int sub = lane / kRun, chunk = lane % kRun;
+  const unsigned char* mine = base + sub * row_bytes + 16 * chunk;
+  const unsigned to0 = ring + sub * UNIT + ((chunk ^ ((sub & 1) << 2)) << 4);
+  int slot = 0;
+  auto copy = [&](int u) {  // unit u into the ring's next slot; nothing past the piece, the rows or a row's end
+    const long long at = static_cast<long long>(u) * UNIT;
+    const bool in = u < u1 && base && at + 16 * chunk < row_bytes;
+    const unsigned to = to0 + slot * kSlot;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (s < s_end && 4 * s + i < srow) {
-            if (has0) v[i] = __ldg(scales + g * srow + 4 * s + i);
-            if (has1) v[4 + i] = __ldg(scales + (g + 8) * srow + 4 * s + i);
-          }
-        f0[j] = make_uint2(v[0] | static_cast<unsigned>(v[1]) << 16, v[2] | static_cast<unsigned>(v[3]) << 16);
-        f1[j] = make_uint2(v[4] | static_cast<unsigned>(v[5]) << 16, v[6] | static_cast<unsigned>(v[7]) << 16);
+    for (int j = 0; j < 16; j += kRowsAtOnce) {
+      const bool there = in && j + sub < rows;
+      copy16(to + j * UNIT, there ? static_cast<const void*>(mine + at + j * row_bytes) : p.x, there);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
+  };
+  // E2M1: the scales of rows g and g + 8 for the four steps of a unit, a unit ahead in registers.
+  const int srow = p.k / 32;  // scales of a row, four to a step
+  const unsigned short* q0 = scales + static_cast<long long>(g) * srow;
+  const unsigned short* q1 = q0 + 8ll * srow;
+  const bool scales_vec = (srow & 3) == 0 && (reinterpret_cast<uintptr_t>(scales) & 7) == 0;
+  constexpr int kHeld = KIND == AD_FP4 ? kUnitSteps : 1;
+  uint2 next0[kHeld], next1[kHeld];
+  auto fetch_scales = [&](int u) {
+    if constexpr (KIND == AD_FP4) {
+#pragma unroll
+      for (int j = 0; j < kUnitSteps; ++j) {
+        const int i0 = 4 * (u * kUnitSteps + j);
+        next0[j] = next1[j] = make_uint2(0u, 0u);
+        if (scales_vec) {
+          if (u < u1 && i0 < srow && has0) next0[j] = __ldg(reinterpret_cast<const uint2*>(q0 + i0));
+          if (u < u1 && i0 < srow && has1) next1[j] = __ldg(reinterpret_cast<const uint2*>(q1 + i0));
+        } else {
+          unsigned short v[8] = {};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (u < u1 && i0 + i < srow) {
+              if (has0) v[i] = __ldg(q0 + i0 + i);
+              if (has1) v[4 + i] = __ldg(q1 + i0 + i);
+            }
+          next0[j] = make_uint2(v[0] | static_cast<unsigned>(v[1]) << 16, v[2] | static_cast<unsigned>(v[3]) << 16);
+          next1[j] = make_uint2(v[4] | static_cast<unsigned>(v[5]) << 16, v[6] | static_cast<unsigned>(v[7]) << 16);
+        }
       }
     }
   };
 #pragma unroll
-  for (int j = 0; j < kAsAhead; ++j) load(2 * u0 + j, j);
+  for (int j = 0; j < DEPTH; ++j) copy(u0 + j);
+  fetch_scales(u0);
+  const int s_end = kUnitSteps * u1;
   if (first) {  // the first weights are asked for before the previous kernel has ended
     grid_dependency_wait();
     grid_launch_dependents();
   }
-  for (int s0 = 2 * u0; s0 < s_end; s0 += kSteps) {
+  for (int s0 = kUnitSteps * u0; s0 < s_end; s0 += kSteps) {
     const int steps = min(kSteps, s_end - s0);
     // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t)
     __syncthreads();  // the last window is read
     if (KIND != AD_BF16 && tid < kAsTokens) top[tid] = 0;
     if (KIND != AD_BF16) __syncthreads();
     const int pieces = steps * P * NB * 32;
-    auto column = [&](int i) {
+    auto fetch = [&](int i) {
       const int ln = i & 31, piece = (i >> 5) / NB % P, s = (i >> 5) / (NB * P);
-      return COLS * (s0 + s) + (KIND == AD_I8 ? 16 * (ln & 3) + 8 * piece : 32 * piece + 8 * (ln & 3));
+      const int col = COLS * (s0 + s) + (KIND == AD_I8 ? 16 * (ln & 3) + 8 * piece : 32 * piece + 8 * (ln & 3));
+      const int token = token0 + (i >> 5) % NB * 8 + (ln >> 2);
+      return i < pieces && token < p.m && col < p.k
+                 ? __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token) * p.k + col))
+                 : make_uint4(0u, 0u, 0u, 0u);
     };
-    for (int i = tid; i < pieces; i += kAsThreads) {  // every copy in flight at once; zeros past M and K
-      const int token = token0 + (i >> 5) % NB * 8 + ((i & 31) >> 2), col = column(i);
-      const bool there = token < p.m && col < p.k;
-      const unsigned short* src = there ? p.x + static_cast<long long>(token) * p.k + col : p.x;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(xs) + 16 * i), "l"(src),
-                   "r"(there ? 16 : 0)
-                   : "memory");
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if constexpr (KIND != AD_BF16) {
-      // BF16 -> FP16 times 2^(141 - ef), ef the largest exponent of the token in the window, which lands below 2^15
-      for (int i = tid; i < pieces; i += kAsThreads) {  // this thread's own copies
-        const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
-        const unsigned u[4] = {v.x, v.y, v.z, v.w};
-        unsigned most = 0;
+    constexpr int kBatch = 8;  // loads of x in flight per thread
+    for (int i0 = tid; i0 < pieces; i0 += kBatch * kAsThreads) {
+      uint4 v[kBatch];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = __vmaxu2(most, (u[e] >> 7) & 0x00ff00ffu);
-        int ef = max(most & 0xffffu, most >> 16);
-        ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 1));
-        ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 2));
-        if ((tid & 3) == 0) atomicMax(top + (i >> 5) % NB * 8 + ((i & 31) >> 2), ef);
+      for (int j = 0; j < kBatch; ++j) v[j] = fetch(i0 + j * kAsThreads);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kAsThreads;
+        if (i < pieces) {  // uniform in a warp
+          if constexpr (KIND != AD_BF16) {  // the largest exponent of the token in the window
+            const unsigned u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            unsigned most = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = __vmaxu2(most, (u[e] >> 7) & 0x00ff00ffu);
+            int ef = max(most & 0xffffu, most >> 16);
+            ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 1));
+            ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 2));
+            if ((tid & 3) == 0) atomicMax(top + (i >> 5) % NB * 8 + ((i & 31) >> 2), ef);
+          }
+          reinterpret_cast<uint4*>(xs)[i] = v[j];
+        }
       }
-      __syncthreads();
+    }
+    __syncthreads();
+    if constexpr (KIND != AD_BF16) {  // BF16 -> FP16 times 2^(141 - ef): the largest lands below 2^15
       for (int i = tid; i < pieces; i += kAsThreads) {
         const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
         unsigned u[4] = {v.x, v.y, v.z, v.w};
@@ -295,70 +338,83 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
         }
         reinterpret_cast<uint4*>(xs)[i] = make_uint4(u[0], u[1], u[2], u[3]);
       }
+      __syncthreads();
     }
-    __syncthreads();
     // ---- the window's steps
     float acc[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[b][e] = 0.0f;
-    const unsigned xa = smem_addr(xs) + 16 * lane;
-    for (int s = 0; s < steps; s += kAsAhead) {
+    unsigned at = smem_addr(xs) + 16 * lane;
+    for (int s = 0; s < steps; s += kUnitSteps, at += kUnitSteps * kStepBytes) {
+      const int unit = (s0 + s) / kUnitSteps;
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      __syncwarp();  // every lane's copies of the unit
+      const unsigned from = ring + slot * kSlot + g * UNIT;
+      uint4 v[kUnitSteps][2];
 #pragma unroll
-      for (int j = 0; j < kAsAhead; ++j) {
-        uint4 v0 = w0[j], v1 = w1[j];
-        uint2 q0, q1;
-        if constexpr (KIND == AD_FP4) q0 = f0[j], q1 = f1[j];
-        load(s0 + s + j + kAsAhead, j);
-        if (s + j < steps) {  // uniform
-          const unsigned at = xa + (s + j) * kStepBytes;
-          if constexpr (KIND == AD_BF16) {
+      for (int j = 0; j < kUnitSteps; ++j) {
+        const unsigned c = ((4 * j + t) ^ ((g & 1) << 2)) << 4;
+        v[j][0] = lds128(from + c), v[j][1] = lds128(from + c + 8 * UNIT);
+      }
+      uint2 now0[kHeld], now1[kHeld];
+      if constexpr (KIND == AD_FP4) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              const uint4 xv = lds128(at + b * 512);
-              const unsigned a0[4] = {v0.x, v1.x, v0.y, v1.y}, a1[4] = {v0.z, v1.z, v0.w, v1.w};
-              mma_bf16(acc[b], a0, xv.x, xv.y);
-              mma_bf16(acc[b], a1, xv.z, xv.w);
-            }
-          } else if constexpr (KIND == AD_I8) {
-            const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
-            uint4 xv[NB][2];
+        for (int j = 0; j < kUnitSteps; ++j) now0[j] = next0[j], now1[j] = next1[j];
+        fetch_scales(unit + 1);
+      }
+      __syncwarp();  // the slot is read
+      copy(unit + DEPTH);
+#pragma unroll
+      for (int j = 0; j < kUnitSteps; ++j) {
+        uint4 v0 = v[j][0], v1 = v[j][1];
+        const unsigned xat = at + j * kStepBytes;
+        if constexpr (KIND == AD_BF16) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint4 xv = lds128(xat + b * 512);
+            const unsigned a0[4] = {v0.x, v1.x, v0.y, v1.y}, a1[4] = {v0.z, v1.z, v0.w, v1.w};
+            mma_bf16(acc[b], a0, xv.x, xv.y);
+            mma_bf16(acc[b], a1, xv.z, xv.w);
+          }
+        } else if constexpr (KIND == AD_I8) {
+          const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
+          uint4 xv[NB][2];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) xv[b][i] = lds128(xat + (i * NB + b) * 512);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            unsigned a[4];
+            i8_pairs(c0[i], a[0], a[2]);
+            i8_pairs(c1[i], a[1], a[3]);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
+              mma_f16(acc[b], a, i & 1 ? xv[b][i >> 1].z : xv[b][i >> 1].x, i & 1 ? xv[b][i >> 1].w : xv[b][i >> 1].y);
+          }
+        } else {
+          transpose_quad(v0, t);
+          transpose_quad(v1, t);
+          const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
+          const unsigned g0[2] = {now0[j].x, now0[j].y}, g1[2] = {now1[j].x, now1[j].y};
 #pragma unroll
-              for (int i = 0; i < 2; ++i) xv[b][i] = lds128(at + (i * NB + b) * 512);
+          for (int i = 0; i < 4; ++i) {  // group i of the step: columns 8 t .. 8 t + 7 of it
+            const unsigned a0[4] = {e2m1x2_to_f16x2(c0[i] & 0xffu), e2m1x2_to_f16x2(c1[i] & 0xffu),
+                                    e2m1x2_to_f16x2(c0[i] >> 8 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 8 & 0xffu)};
+            const unsigned a1[4] = {e2m1x2_to_f16x2(c0[i] >> 16 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 16 & 0xffu),
+                                    e2m1x2_to_f16x2(c0[i] >> 24), e2m1x2_to_f16x2(c1[i] >> 24)};
+            const float h0 = f16_to_f32(static_cast<unsigned short>(g0[i >> 1] >> (16 * (i & 1))));
+            const float h1 = f16_to_f32(static_cast<unsigned short>(g1[i >> 1] >> (16 * (i & 1))));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              unsigned a[4];
-              i8_pairs(c0[i], a[0], a[2]);
-              i8_pairs(c1[i], a[1], a[3]);
-#pragma unroll
-              for (int b = 0; b < NB; ++b)
-                mma_f16(acc[b], a, i & 1 ? xv[b][i >> 1].z : xv[b][i >> 1].x, i & 1 ? xv[b][i >> 1].w : xv[b][i >> 1].y);
-            }
-          } else {
-            transpose_quad(v0, t);
-            transpose_quad(v1, t);
-            const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
-            const unsigned g0[2] = {q0.x, q0.y}, g1[2] = {q1.x, q1.y};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // group i of the step: columns 8 t .. 8 t + 7 of it
-              const unsigned a0[4] = {e2m1x2_to_f16x2(c0[i] & 0xffu), e2m1x2_to_f16x2(c1[i] & 0xffu),
-                                      e2m1x2_to_f16x2(c0[i] >> 8 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 8 & 0xffu)};
-              const unsigned a1[4] = {e2m1x2_to_f16x2(c0[i] >> 16 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 16 & 0xffu),
-                                      e2m1x2_to_f16x2(c0[i] >> 24), e2m1x2_to_f16x2(c1[i] >> 24)};
-              const float h0 = f16_to_f32(static_cast<unsigned short>(g0[i >> 1] >> (16 * (i & 1))));
-              const float h1 = f16_to_f32(static_cast<unsigned short>(g1[i >> 1] >> (16 * (i & 1))));
-#pragma unroll
-              for (int b = 0; b < NB; ++b) {
-                const uint4 xv = lds128(at + (i * NB + b) * 512);
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_f16(d, a0, xv.x, xv.y);
-                mma_f16(d, a1, xv.z, xv.w);
-                acc[b][0] = fma_rn(d[0], h0, acc[b][0]), acc[b][1] = fma_rn(d[1], h0, acc[b][1]);
-                acc[b][2] = fma_rn(d[2], h1, acc[b][2]), acc[b][3] = fma_rn(d[3], h1, acc[b][3]);
-              }
+            for (int b = 0; b < NB; ++b) {
+              const uint4 xv = lds128(xat + (i * NB + b) * 512);
+              float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma_f16(d, a0, xv.x, xv.y);
+              mma_f16(d, a1, xv.z, xv.w);
+              acc[b][0] = fma_rn(d[0], h0, acc[b][0]), acc[b][1] = fma_rn(d[1], h0, acc[b][1]);
+              acc[b][2] = fma_rn(d[2], h1, acc[b][2]), acc[b][3] = fma_rn(d[3], h1, acc[b][3]);
             }
           }
         }
@@ -376,6 +432,8 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
         }
       }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");  // what is left copied nothing
+  __syncwarp();  // the ring is free for the next piece
 }
 
 template <int KIND, int NB>
@@ -384,6 +442,7 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
   __shared__ int top[kAsTokens];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int tile = blockIdx.y, token0 = tile * kAsTokens;
+  const unsigned ring = smem_addr(xs) + kAsWindow + warp * as_depth(KIND) * as_slot(KIND);
   const int a_total = p.a_blocks * p.a_units, total = a_total + p.w_blocks * p.w_units;
   int pos = min(static_cast<long long>(blockIdx.x) * p.share, static_cast<long long>(total));
   const int end = min(pos + p.share, total);
@@ -412,7 +471,7 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       const unsigned char* base = has ? reinterpret_cast<const unsigned char*>(
                                             p.a + (static_cast<long long>(id) * p.rank + 16 * rg) * p.k)
                                       : nullptr;
-      stream_piece<AD_BF16, NB>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1, token0, xs, top, sum, false);
+      stream_piece<AD_BF16, NB, as_unit(KIND), as_depth(KIND)>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1, token0, xs, ring, top, sum, false);
       if (has) {
         const int column = token - token0;
         float* to = p.a_part + ((static_cast<long long>(tile) * p.a_blocks + block) * p.a_pieces + piece) * kAsRows + 16 * warp;
@@ -426,8 +485,8 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       const int row0 = block * kAsRows + 16 * warp, rows = p.n - row0;
       const unsigned short* scales =
           KIND == AD_FP4 ? static_cast<const unsigned short*>(p.side) + static_cast<long long>(row0) * (p.k / 32) : nullptr;
-      stream_piece<KIND, NB>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes, scales, rows, u0, u1, token0, xs,
-                             top, sum, first);
+      stream_piece<KIND, NB, as_unit(KIND), as_depth(KIND)>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes, scales, rows, u0, u1, token0, xs,
+                             ring, top, sum, first);
       first = false;
       const int tokens = min(kAsTokens, p.m - token0);
       float* to = p.w_part + (((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces + piece) * kAsTokens) * kAsRows +
@@ -537,8 +596,8 @@ StreamPlan plan_stream(int kind, StreamParams& p, int places) {
   const int tokens = p.m < kAsTokens ? p.m : kAsTokens;
   p.a_blocks = (tokens * p.groups + kAsWarps - 1) / kAsWarps;
   p.w_blocks = (p.n + kAsRows - 1) / kAsRows;
-  p.a_units = static_cast<int>((2ll * p.k + kAsUnit - 1) / kAsUnit);
-  p.w_units = static_cast<int>((p.row_bytes + kAsUnit - 1) / kAsUnit);
+  p.a_units = static_cast<int>((2ll * p.k + as_unit(kind) - 1) / as_unit(kind));
+  p.w_units = static_cast<int>((p.row_bytes + as_unit(kind) - 1) / as_unit(kind));
   const long long total = static_cast<long long>(p.a_blocks) * p.a_units + static_cast<long long>(p.w_blocks) * p.w_units;
   const long long share = (total + places - 1) / places;
   p.share = static_cast<int>(share < kAsMinShare ? kAsMinShare : share);
@@ -572,11 +631,11 @@ int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t strea
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (!(ready.load() >> dev & 1)) {
-    err = cudaFuncSetAttribute(adapter_stream_kernel<KIND, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAsWindow);
+    err = cudaFuncSetAttribute(adapter_stream_kernel<KIND, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, as_smem(KIND));
     if (err != cudaSuccess) return err;
     ready.fetch_or(1ull << dev);
   }
-  const int rc = launch_stream(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, kAsWindow, p, stream);
+  const int rc = launch_stream(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, as_smem(KIND), p, stream);
   if (rc) return rc;
   return launch_stream(adapter_join_kernel<KIND>, dim3(p.w_blocks, p.m), kAsRows, 0, p,
                        stream);

@@ -189,6 +189,67 @@ def test_store_and_read_match_the_format(dim, heads, page, dtype, tokens):
                 assert np.array_equal(new & bits, want & bits)
 
 
+@pytest.mark.parametrize("dim,heads,page,dtype,tokens", [(64, 9, 16, "bf16", 2049), (128, 8, 64, "fp16", 1025), (128, 9, 16, "bf16", 3641),
+                                                         (128, 16, 64, "fp16", 2049), (256, 5, 32, "bf16", 3500)])
+@pytest.mark.parametrize("order", ["runs", "shuffled", "backwards"])
+def test_many_rows_give_what_few_rows_give(dim, heads, page, dtype, tokens, order):
+    """One call over many rows against calls over 64: the same bytes, the same rows back."""
+    from klab_b200 import kv_pages
+
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    pages = tokens // page + 3
+    slots = torch.arange(3, tokens + 3, device="cuda", dtype=torch.int32)
+    if order == "shuffled":
+        slots = torch.randperm(pages * page, device="cuda", generator=g)[:tokens].int()
+    elif order == "backwards":
+        slots = slots.flip(0).contiguous()
+    slots[torch.rand(tokens, device="cuda", generator=g) < 0.05] = -1
+    # Rows on 16 bytes, and (of heads of an odd number) on 8: both ways to load.
+    for pad in (0, 4):
+        kv = torch.randn(tokens, 2, heads * dim + pad, device="cuda", generator=g).to(DT[dtype])
+        kv[7, 0, 40] = float("nan")
+        kv[8, 1, 3] = float("inf")
+        kv[9] = 0
+        kv[10] *= 2.0 ** -20
+        k, v = (kv[:, i, :heads * dim].unflatten(1, (heads, dim)) for i in (0, 1))
+        many = torch.randint(0, 256, (pages, heads, kv_pages.page_bytes(page, dim)), dtype=torch.uint8, device="cuda", generator=g)
+        few = many.clone()
+        kv_pages.store(k, v, many, slots)
+        for at in range(0, tokens, 64):
+            kv_pages.store(k[at:at + 64], v[at:at + 64], few, slots[at:at + 64])
+        assert torch.equal(many, few)
+        for out in (torch.bfloat16, torch.float16, torch.float32):
+            whole = kv_pages.read(many, slots, dim, dtype=out)
+            for at in range(0, tokens, 64):
+                for a, b in zip(whole, kv_pages.read(many, slots[at:at + 64], dim, dtype=out)):
+                    assert torch.equal(a[at:at + 64], b)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scales_and_codes_of_every_largest_value(dtype):
+    """Groups whose max|x| takes every 16-bit pattern from 0 to infinity, at both ways to store."""
+    from klab_b200 import kv_pages
+
+    tokens, heads, dim, page = 4096, 8, 128, 64
+    top = torch.arange(tokens * heads * 4).div(4, rounding_mode="floor").clamp(max=0x7f80 if dtype == "bf16" else 0x7c00).to(torch.int16).view(DT[dtype])
+    top = top.double().nan_to_num().view(tokens, heads, 4, 1)
+    part = torch.arange(32) / 14.0 * torch.tensor([1, -1]).repeat(16)  # 0 and near the halves of a step up to the largest
+    x = top * part.clamp(-1, 1)
+    x[..., 31:] = top
+    x = x.to(DT[dtype]).flatten(2)
+    codes, scales = ok.quantize(x.double().numpy())
+    want = ok.values(codes, scales)
+    slots = i32(np.arange(tokens))
+    buf = kv_pages.empty_pages(tokens // page, heads, page, dim)
+    dev = x.cuda()
+    for step in (tokens, 128):
+        buf.zero_()
+        for at in range(0, tokens, step):
+            kv_pages.store(dev[at:at + step], -dev[at:at + step], buf, slots[at:at + step])
+        k, v = kv_pages.read(buf, slots, dim, dtype=torch.float32)
+        assert np.array_equal(f64(k), want) and np.array_equal(f64(v), -want)
+
+
 def test_slots_outside_the_pages_touch_nothing(native):
     from klab_b200 import kv_pages
 

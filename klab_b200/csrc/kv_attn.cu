@@ -29,8 +29,11 @@
 // Scores beyond a row's last position are -inf before the softmax, and the scales of tokens beyond the request are zeroed,
 // so whatever the allocator left there (NaN scales included) has no part.
 //
-// What bounds it: long caches the issue slots (about 470 instructions a warp and unit of 4608 bytes at D = 128, IPC 2.3),
-// before HBM; short ones launch and dependent loads (lengths, table, first block).
+// What bounds it: long caches the warps' own chains (about 490 instructions a warp and unit of 4608 bytes at D = 128, IPC
+// 1.7 with the 12 warps that registers allow, the ALU pipe at 48 %), before HBM: 64 x 8192 tokens, 8 kv heads of 128,
+// 243 MB in 60.6 us, 4.0 TB/s; 1 x 131072, 151 MB in 36.6 us, 4.1 TB/s. Four CTAs an SM (80 registers), more shares than
+// CTAs, the next piece's first copies issued ahead and 16 rows a tile all measured the same or slower. Short ones launch,
+// dependent loads (lengths, table, first block) and the join (2.8 us): 1 x 300 tokens 4.9 us.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -48,19 +51,16 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 8;  // query rows of a tile (the MMA's N)
-#ifndef KLAB_KV_SLOTS
-#define KLAB_KV_SLOTS 2  // units of two blocks that a warp's ring holds
-#endif
-constexpr int kSlots = KLAB_KV_SLOTS;
-#ifndef KLAB_KV_MIN_SHARE
-#define KLAB_KV_MIN_SHARE 4  // units a CTA takes at least
-#endif
-constexpr int kMinShare = KLAB_KV_MIN_SHARE;
+// Units of two blocks that a warp's ring holds: a third one takes shared memory and L1 from the third CTA of an SM at heads
+// of 64 and 256 (25.9 us against 33.6, 23.1 against 31.7) and changes heads of 128 by 1 %.
+constexpr int kSlots = 2;
+// Units a CTA takes at least: short batches pay for the sums that every share leaves (8 x 2048 drafts 13.8 us, with 8 units
+// 15.1; 1 x 2000 tokens 7.7 us, with 2 units 8.3, with 8 units 7.9).
+constexpr int kMinShare = 4;
 constexpr int kUnitTokens = 2 * kKvBlock;
-#ifndef KLAB_KV_WHOLE
-#define KLAB_KV_WHOLE 16
-#endif
-constexpr int kWholeUnits = KLAB_KV_WHOLE;
+// Tables of at most this many units are not cut: 1 x 250 tokens 4.9 us against 6.5 cut, 64 x 512 14.6 against 18.7;
+// 1 x 2000 16.6 us whole and 7.7 cut.
+constexpr int kWholeUnits = 16;
 constexpr float kNegInf = -__builtin_huge_valf();
 // A row's weights are 2^(score - ref) with ref = (a score near the largest) - 10, moved when a score passes it by 2^14; V
 // scales below 2 then keep P' below 2^15.
@@ -254,11 +254,8 @@ __device__ __forceinline__ void next_segment(const KvAttnParams& p, Share& it) {
   } while (it.r.tiles == 0 && it.request + 1 < p.requests);
 }
 
-#ifndef KLAB_KV_RESIDENT
-#define KLAB_KV_RESIDENT 3
-#endif
-// CTAs per SM the registers are cut for.
-constexpr int kv_resident(int ng) { return ng <= 4 ? KLAB_KV_RESIDENT : 2; }
+// CTAs per SM the registers are cut for; heads of 256 hold twice the accumulators.
+constexpr int kv_resident(int ng) { return ng <= 4 ? 3 : 2; }
 
 __device__ __forceinline__ long long record_of(const KvAttnParams& p, int cta, int kvh, int which) {
   return ((static_cast<long long>(cta) * p.kv_heads + kvh) * 2 + which) * kRows;
@@ -443,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
       live = __all_sync(0xffffffffu, live);
       if (!live) {  // leave, after a bounded wait for the warp's other copies in flight
         if (lane == 0) record_status(p.status, kStatusMbarTimeout);
-        for (int k = s + 1; k < count && k < s + kSlots; ++k) 
+        for (int k = s + 1; k < count && k < s + kSlots; ++k)
           (void)mbar_wait(bar0 + 8 * ((turn + k) % kSlots), (turn + k) / kSlots & 1);
         break;
       }

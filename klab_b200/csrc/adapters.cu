@@ -278,14 +278,20 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
       }
     }
   };
+  // Before the previous kernel has ended only L2 is asked for the first units: it may still be writing them.
+  if (first) {
+    if (base && lane < min(rows, 16)) {
+      const long long at = static_cast<long long>(u0) * UNIT, left = row_bytes - at;
+      bulk_prefetch_l2(base + lane * row_bytes + at,
+                       static_cast<unsigned>(min(left, static_cast<long long>(min(DEPTH, u1 - u0) * UNIT))));
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
 #pragma unroll
   for (int j = 0; j < DEPTH; ++j) copy(u0 + j);
   fetch_scales(u0);
   const int s_end = kUnitSteps * u1;
-  if (first) {  // the first weights are asked for before the previous kernel has ended
-    grid_dependency_wait();
-    grid_launch_dependents();
-  }
   for (int s0 = kUnitSteps * u0; s0 < s_end; s0 += kSteps) {
     const int steps = min(kSteps, s_end - s0);
     // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t)

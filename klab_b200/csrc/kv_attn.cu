@@ -180,48 +180,58 @@ struct Share {
 };
 
 __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int ctas, bool report) {
-  constexpr int kEach = 4;  // chunks of 32 requests whose loads are in flight at once
-  const int lane = threadIdx.x & 31;
+  constexpr int kFlight = 4;  // requests of a lane whose loads are in flight at once
+  const int lane = threadIdx.x & 31, each = (p.requests + 31) / 32;
   bool bad = false;
-  auto load = [&](int base) {
-    const int i = base + lane;
-    int length = 0, start = 0, end = 0;
-    if (i < p.requests) {
+  auto load = [&](int i, int end) {
+    int length = 0, start = 0, stop = 0;
+    if (i < end) {
       length = __ldg(p.lengths + i);
       start = __ldg(p.starts + i);
-      end = __ldg(p.starts + i + 1);
+      stop = __ldg(p.starts + i + 1);
     }
-    return make_request(p, length, start, end, bad);
+    return make_request(p, length, start, stop, bad);
   };
-  Request r = load(0);  // lane's request of a chunk
-  int all = r.tiles * r.units;
-  for (int base = 32; base < p.requests; base += 32 * kEach) {
+  auto scan = [&](int upto) {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      if (base + 32 * j < p.requests) {
-        const Request q = load(base + 32 * j);
-        all += q.tiles * q.units;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += up;
+    }
+    return upto;
+  };
+  // A lane adds up a run of `each` requests; the run that holds the share's beginning is then looked through by all.
+  Request r = load(lane * each, p.requests);
+  int mine = r.tiles * r.units;
+  for (int j = 1; j < each; j += kFlight) {
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (j + u < each) {
+        const Request q = load(lane * each + j + u, p.requests);
+        mine += q.tiles * q.units;
       }
   }
-  all = __reduce_add_sync(0xffffffffu, all);
-  if (bad && report) record_status(p.status, kStatusBadLength);
+  int upto = scan(mine);
+  const int all = __shfl_sync(0xffffffffu, upto, 31);
+  if (__any_sync(0xffffffffu, bad) && report) record_status(p.status, kStatusBadLength);
   Share it;
   it.share = max(p.whole ? 1 : kMinShare, (all + ctas - 1) / ctas);
   it.pos = min(static_cast<long long>(cta) * it.share, static_cast<long long>(all));
   it.end = min(it.pos + it.share, all);
   it.request = it.tile = it.unit = 0;
   if (it.pos >= it.end) return it;
-  int left = it.pos;  // units from the start of the chunk
-  for (int base = 0;; r = load(base += 32)) {
-    const int mine = r.tiles * r.units;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += up;
-    }
-    const int before = upto - mine;
-    const unsigned owner = __ballot_sync(0xffffffffu, left >= before && left < upto);
+  int left = it.pos;  // units from the start of what `upto` counts
+  int base = 0, stop = p.requests;
+  if (each > 1) {
+    const int from = __ffs(__ballot_sync(0xffffffffu, left < upto)) - 1;
+    left -= __shfl_sync(0xffffffffu, upto - mine, from);
+    base = from * each, stop = min(base + each, p.requests);
+    r = load(base + lane, stop);
+    mine = r.tiles * r.units;
+    upto = scan(mine);
+  }
+  while (true) {
+    const unsigned owner = __ballot_sync(0xffffffffu, left < upto);
     if (owner) {
       const int from = __ffs(owner) - 1;
       it.request = base + from;
@@ -230,7 +240,7 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
       it.r.token0 = __shfl_sync(0xffffffffu, r.token0, from);
       it.r.tiles = __shfl_sync(0xffffffffu, r.tiles, from);
       it.r.units = __shfl_sync(0xffffffffu, r.units, from);
-      it.unit = left - __shfl_sync(0xffffffffu, before, from);
+      it.unit = left - __shfl_sync(0xffffffffu, upto - mine, from);
       if (it.r.tiles > 1) {
         it.tile = it.unit / it.r.units;
         it.unit -= it.tile * it.r.units;
@@ -238,6 +248,14 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
       return it;
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
+    base += 32;
+    if (base >= stop) {  // not with lengths that stay as they are during the call
+      it.pos = it.end;
+      return it;
+    }
+    r = load(base + lane, stop);
+    mine = r.tiles * r.units;
+    upto = scan(mine);
   }
 }
 
@@ -247,11 +265,10 @@ __device__ __forceinline__ void next_segment(const KvAttnParams& p, Share& it) {
   if (++it.tile < it.r.tiles) return;
   it.tile = 0;
   bool bad = false;
-  do {
-    ++it.request;
-    it.r = make_request(p, __ldg(p.lengths + it.request), __ldg(p.starts + it.request),
-                              __ldg(p.starts + it.request + 1), bad);
-  } while (it.r.tiles == 0 && it.request + 1 < p.requests);
+  it.r.tiles = 0;
+  while (it.r.tiles == 0 && ++it.request < p.requests)
+    it.r = make_request(p, __ldg(p.lengths + it.request), __ldg(p.starts + it.request), __ldg(p.starts + it.request + 1), bad);
+  if (it.r.tiles == 0) it.pos = it.end;  // not with lengths that stay as they are during the call
 }
 
 // CTAs per SM the registers are cut for; heads of 256 hold twice the accumulators.

@@ -116,6 +116,36 @@ def test_not_a_number_stays_in_its_row():
         assert y[0].isnan().all() and torch.equal(y[1:], clean[1:])
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_weights_that_the_call_before_wrote(captured):
+    """Rows out of one call are the weights of the next, with nothing between the two on the stream."""
+    from klab_b200.adapters import adapter_linear
+
+    w, _, x, a, b, c, ids = case("bf16", 192, 1024, 512, 16, 3)
+    _, _, x2, a2, b2, c2, ids2 = case("bf16", 5, 192, 1024, 16, 2, seed=1)
+    xs = [x, x * 2, x * -1, x.roll(1, 0)]
+    want = []
+    for v in xs:
+        y = adapter_linear(v, w, a, b, c, ids)
+        torch.cuda.synchronize()
+        want.append(adapter_linear(x2, y, a2, b2, c2, ids2))
+    y = torch.zeros_like(y)  # one buffer that every pair writes anew
+
+    def run():
+        return [adapter_linear(x2, adapter_linear(v, w, a, b, c, ids, out=y), a2, b2, c2, ids2) for v in xs * 4]
+
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run()
+        for _ in range(3):
+            g.replay()
+    else:
+        got = run()
+    for i, v in enumerate(got):
+        assert torch.equal(v, want[i % len(xs)])
+
+
 def test_graphs_and_streams():
     from klab_b200.adapters import adapter_linear
 

@@ -304,7 +304,7 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
       const int col = COLS * (s0 + s) + (KIND == AD_I8 ? 16 * (ln & 3) + 8 * piece : 32 * piece + 8 * (ln & 3));
       const int token = token0 + (i >> 5) % NB * 8 + (ln >> 2);
       return i < pieces && token < p.m && col < p.k
-                 ? __ldg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token) * p.k + col))
+                 ? __ldcg(reinterpret_cast<const uint4*>(p.x + static_cast<long long>(token) * p.k + col))
                  : make_uint4(0u, 0u, 0u, 0u);
     };
     constexpr int kBatch = 8;  // loads of x in flight per thread
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       }
       const int group = block * kAsWarps + warp, token = token0 + group / p.groups, rg = group % p.groups;
       const bool there = group < kAsTokens * p.groups && token < p.m;
-      const int id = there ? __ldg(p.ids + token) : -1;
+      const int id = there ? __ldcg(p.ids + token) : -1;
       const bool has = id >= 0 && id < p.adapters;
       if (there && !has && id != -1 && lane == 0) record_status(p.status, kStatusBadAdapter);
       const unsigned char* base = has ? reinterpret_cast<const unsigned char*>(
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
   const int tid = threadIdx.x, block = blockIdx.x, row = block * kAsRows + tid, token = blockIdx.y;
   const int tile = token / kAsTokens, slot = token % kAsTokens;
   constexpr int kHeld = 8;  // 16-byte runs of B that are asked for ahead
-  const int id = __ldg(p.ids + token);
+  const int id = __ldcg(p.ids + token);
   const bool has = id >= 0 && id < p.adapters;
   const uint4* b = reinterpret_cast<const uint4*>(p.b + (static_cast<long long>(has ? id : 0) * p.n + min(row, p.n - 1)) * p.rank);
   const int runs = has ? p.rank / 8 : 0;

@@ -183,12 +183,14 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
   constexpr int kFlight = 4;  // requests of a lane whose loads are in flight at once
   const int lane = threadIdx.x & 31, each = (p.requests + 31) / 32;
   bool bad = false;
+  // Ordinary loads, here and for q and the table: what the launch before wrote while this one was already resident is not
+  // read-only data of the kernel.
   auto load = [&](int i, int end) {
     int length = 0, start = 0, stop = 0;
     if (i < end) {
-      length = __ldg(p.lengths + i);
-      start = __ldg(p.starts + i);
-      stop = __ldg(p.starts + i + 1);
+      length = p.lengths[i];
+      start = p.starts[i];
+      stop = p.starts[i + 1];
     }
     return make_request(p, length, start, stop, bad);
   };
@@ -267,7 +269,7 @@ __device__ __forceinline__ void next_segment(const KvAttnParams& p, Share& it) {
   bool bad = false;
   it.r.tiles = 0;
   while (it.r.tiles == 0 && ++it.request < p.requests)
-    it.r = make_request(p, __ldg(p.lengths + it.request), __ldg(p.starts + it.request), __ldg(p.starts + it.request + 1), bad);
+    it.r = make_request(p, p.lengths[it.request], p.starts[it.request], p.starts[it.request + 1], bad);
   if (it.r.tiles == 0) it.pos = it.end;  // not with lengths that stay as they are during the call
 }
 
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
                                 static_cast<long long>(kvh * p.group + at - token * p.group) * D;
 #pragma unroll
     for (int G = 0; G < NG; ++G)
-      qw[G] = row < rows ? __ldg(reinterpret_cast<const uint4*>(src + 32 * G + 8 * t)) : make_uint4(0u, 0u, 0u, 0u);
+      qw[G] = row < rows ? *reinterpret_cast<const uint4*>(src + 32 * G + 8 * t) : make_uint4(0u, 0u, 0u, 0u);
     // Units of two blocks (32 tokens) go to the warps in turn; unit s of this warp begins at block first_block + 2 * (warp +
     // 4 * s).
     const int first_block = 2 * it.unit, last_block = (length + kKvBlock - 1) / kKvBlock;
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
       if (u == 0) {
         const int block = first_block + 2 * (warp + kWarps * (s + (lane >> 1))) + (lane & 1);
         const bool there = block < last_block;
-        const int id = there ? __ldg(table + (block >> per_page_shift)) : -1;
+        const int id = there ? table[block >> per_page_shift] : -1;
         const bool page = id >= 0 && id < p.num_pages;
         if (there && !page) record_status(p.status, kStatusBadPage);
         const long long at =

@@ -175,11 +175,11 @@ __global__ void __launch_bounds__(kStoreThreads) kv_store_kernel(const RowParams
     const auto* ks = static_cast<const unsigned short*>(p.k) + row * p.k_stride + w.head * p.k_head + 8 * w.c;
     const auto* vs = static_cast<const unsigned short*>(p.v) + row * p.v_stride + w.head * p.v_head + 8 * w.c;
     if (p.wide) {
-      k = ldg128_stream(ks);
-      v = ldg128_stream(vs);
+      k = __ldcs(reinterpret_cast<const uint4*>(ks));
+      v = __ldcs(reinterpret_cast<const uint4*>(vs));
     } else {  // rows on 8-byte boundaries
-      const uint2 k0 = __ldg(reinterpret_cast<const uint2*>(ks)), k1 = __ldg(reinterpret_cast<const uint2*>(ks) + 1);
-      const uint2 v0 = __ldg(reinterpret_cast<const uint2*>(vs)), v1 = __ldg(reinterpret_cast<const uint2*>(vs) + 1);
+      const uint2 k0 = *reinterpret_cast<const uint2*>(ks), k1 = *(reinterpret_cast<const uint2*>(ks) + 1);
+      const uint2 v0 = *reinterpret_cast<const uint2*>(vs), v1 = *(reinterpret_cast<const uint2*>(vs) + 1);
       k = make_uint4(k0.x, k0.y, k1.x, k1.y);
       v = make_uint4(v0.x, v0.y, v1.x, v1.y);
     }
@@ -237,7 +237,7 @@ __device__ __forceinline__ Pair pair_of(const RowParams& p, unsigned at) {
 }
 
 __device__ __forceinline__ int slot_of(const RowParams& p, unsigned token) {
-  return token < p.tokens ? __ldg(p.slots + token) : -1;
+  return token < p.tokens ? p.slots[token] : -1;
 }
 
 template <int D>
@@ -295,10 +295,10 @@ __device__ __forceinline__ void read_rows(const void* from, long long stride, lo
       x[i][u] = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);  // skipped: any ordinary value
       if (w.slot[i] == -1) continue;
       if (p.wide) {
-        x[i][u] = ldg128_stream(row + 32 * u);
+        x[i][u] = __ldcs(reinterpret_cast<const uint4*>(row + 32 * u));
       } else {  // rows on 8-byte boundaries
         const uint2* half = reinterpret_cast<const uint2*>(row + 32 * u);
-        const uint2 a = __ldg(half), b = __ldg(half + 1);
+        const uint2 a = half[0], b = half[1];
         x[i][u] = make_uint4(a.x, a.y, b.x, b.y);
       }
     }

@@ -4,8 +4,9 @@
 //
 // Work: a segment is a tile of 8 query rows of a request and kv head (its query heads times its new tokens), in units of
 // 32 tokens. All segments of a kv head, one behind the other, are cut into equal shares, one for each CTA that the machine
-// holds at once; every CTA adds up all requests to find its own, so uneven batches and single long ones fill the machine
-// alike, and its 4 warps take a piece's units in turn. A piece that is not a whole segment leaves its sums in scratch, and
+// holds at once (or, while shares are short, every segment into shares of its own that are nearly as long); every CTA adds
+// up all requests to find its own, so uneven batches and single long ones fill the machine alike, and its 4 warps take a
+// piece's units in turn. A piece that is not a whole segment leaves its sums in scratch, and
 // kv_combine_kernel joins them in order (a second launch, because per-call scratch then needs no zeroed counters: two
 // captured graphs or two streams never share any). Tables of at most 512 tokens a request are not cut: whole segments are
 // dealt, and the second launch is saved.
@@ -57,6 +58,11 @@ constexpr int kSlots = 2;
 // Units a CTA takes at least: short batches pay for the sums that every share leaves (8 x 2048 drafts 13.8 us, with 8 units
 // 15.1; 1 x 2000 tokens 7.7 us, with 2 units 8.3, with 8 units 7.9).
 constexpr int kMinShare = 4;
+// Up to 64 requests whose equal shares have at most kTry units: every segment gets CTAs of its own where shares of up to
+// kSlack units more allow it, since a CTA's second piece starts and ends like its first: 16 x 4096 tokens 14.0 us, with
+// equal shares 16.6; 32 x 1000 12.4 and 18.3; 8 x 2048 drafts 12.1 and 14.2. Above kTry equal shares are as good or better
+// (32 x 8192 35.4 us; 36.1 with the search), and 8 units of slack leave out little (32 x 4096 25.9 us, 16 units 25.6).
+constexpr int kTry = 40, kSlack = 16;
 constexpr int kUnitTokens = 2 * kKvBlock;
 // Tables of at most this many units are not cut: 1 x 250 tokens 4.9 us against 6.5 cut, 64 x 512 14.6 against 18.7;
 // 1 x 2000 16.6 us whole and 7.7 cut.
@@ -174,8 +180,9 @@ __device__ __forceinline__ Request make_request(const KvAttnParams& p, int lengt
 // Units of all (request, tile) one behind the other, requests in order; a CTA takes `share` of them from `pos` on. Every
 // warp works its piece out for itself: the loads are the same few lines for the whole machine, and no barrier is needed.
 struct Share {
-  int pos, end, share;       // this CTA's units
+  int pos, end;              // this CTA's units
   int request, tile, unit;   // the segment that holds `pos`, and the unit within it
+  int first, last;           // the CTAs that this segment's units went to
   Request r;
 };
 
@@ -203,9 +210,9 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
     return upto;
   };
   // A lane adds up a run of `each` requests; the run that holds the share's beginning is then looked through by all.
-  Request r = load(lane * each, p.requests);
-  int mine = r.tiles * r.units;
-  for (int j = 1; j < each; j += kFlight) {
+  Request held[2] = {load(lane * each, p.requests), load(lane * each + 1, each > 1 ? p.requests : 0)};
+  int mine = held[0].tiles * held[0].units + held[1].tiles * held[1].units;
+  for (int j = 2; j < each; j += kFlight) {
 #pragma unroll
     for (int u = 0; u < kFlight; ++u)
       if (j + u < each) {
@@ -217,13 +224,64 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
   const int all = __shfl_sync(0xffffffffu, upto, 31);
   if (__any_sync(0xffffffffu, bad) && report) record_status(p.status, kStatusBadLength);
   Share it;
-  it.share = max(p.whole ? 1 : kMinShare, (all + ctas - 1) / ctas);
-  it.pos = min(static_cast<long long>(cta) * it.share, static_cast<long long>(all));
-  it.end = min(it.pos + it.share, all);
-  it.request = it.tile = it.unit = 0;
+  it.request = it.tile = it.unit = it.first = it.last = 0;
+  auto take = [&](const Request& r, int from) {
+    it.r.length = __shfl_sync(0xffffffffu, r.length, from);
+    it.r.fresh = __shfl_sync(0xffffffffu, r.fresh, from);
+    it.r.token0 = __shfl_sync(0xffffffffu, r.token0, from);
+    it.r.tiles = __shfl_sync(0xffffffffu, r.tiles, from);
+    it.r.units = __shfl_sync(0xffffffffu, r.units, from);
+  };
+  const int share = max(p.whole ? 1 : kMinShare, (all + ctas - 1) / ctas);
+  if (each <= 2 && !p.whole && share <= kTry && (p.requests > 1 || p.max_new * p.group > kRows) &&
+      __reduce_add_sync(0xffffffffu, held[0].tiles + held[1].tiles) <= ctas) {
+    // CTAs of its own for every segment: a lane counts them for shares of share + lane units.
+    const float by = 1.0f / static_cast<float>(share + lane);
+    int need = 0;
+    auto count_of = [&](const Request& r, int i) {
+      return __shfl_sync(0xffffffffu, r.tiles, i) *
+             static_cast<int>(ceilf(static_cast<float>(__shfl_sync(0xffffffffu, r.units, i)) * by));
+    };
+#pragma unroll 4
+    for (int i = 0; i < min(p.requests, 32); ++i) need += count_of(held[0], i);
+    if (each > 1) {
+#pragma unroll 4
+      for (int i = 0; i < 32; ++i) need += count_of(held[1], i);
+    }
+    const unsigned fits = __ballot_sync(0xffffffffu, lane <= kSlack && need <= ctas);
+    if (fits) {
+      const int own = share + __ffs(fits) - 1;
+      int parts[2], count[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) parts[j] = (held[j].units + own - 1) / own, count[j] = held[j].tiles * parts[j];
+      const int behind = scan(count[0] + count[1]), total = __shfl_sync(0xffffffffu, behind, 31);
+      if (total <= ctas) {
+        it.pos = it.end = 0;
+        const unsigned owner = __ballot_sync(0xffffffffu, cta < behind);
+        if (!owner) return it;  // a CTA too many
+        const int from = __ffs(owner) - 1, before = __shfl_sync(0xffffffffu, behind - count[0] - count[1], from);
+        const int second = cta - before >= __shfl_sync(0xffffffffu, count[0], from);
+        const int rest = cta - before - (second ? __shfl_sync(0xffffffffu, count[0], from) : 0);
+        const int n = __shfl_sync(0xffffffffu, second ? parts[1] : parts[0], from);
+        Request r = held[0];
+        if (second) r = held[1];
+        take(r, from);
+        it.request = from * each + second;
+        it.tile = rest / n;
+        const int part = rest - it.tile * n;
+        it.unit = part * it.r.units / n;  // n shares of at most kTry + kSlack units: the product is small
+        it.end = (part + 1) * it.r.units / n - it.unit;
+        it.first = cta - part, it.last = it.first + n - 1;
+        return it;
+      }
+    }
+  }
+  it.pos = min(static_cast<long long>(cta) * share, static_cast<long long>(all));
+  it.end = min(it.pos + share, all);
   if (it.pos >= it.end) return it;
   int left = it.pos;  // units from the start of what `upto` counts
   int base = 0, stop = p.requests;
+  Request r = held[0];
   if (each > 1) {
     const int from = __ffs(__ballot_sync(0xffffffffu, left < upto)) - 1;
     left -= __shfl_sync(0xffffffffu, upto - mine, from);
@@ -237,16 +295,14 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
     if (owner) {
       const int from = __ffs(owner) - 1;
       it.request = base + from;
-      it.r.length = __shfl_sync(0xffffffffu, r.length, from);
-      it.r.fresh = __shfl_sync(0xffffffffu, r.fresh, from);
-      it.r.token0 = __shfl_sync(0xffffffffu, r.token0, from);
-      it.r.tiles = __shfl_sync(0xffffffffu, r.tiles, from);
-      it.r.units = __shfl_sync(0xffffffffu, r.units, from);
+      take(r, from);
       it.unit = left - __shfl_sync(0xffffffffu, upto - mine, from);
       if (it.r.tiles > 1) {
         it.tile = it.unit / it.r.units;
         it.unit -= it.tile * it.r.units;
       }
+      const int begin = it.pos - it.unit;
+      it.first = begin / share, it.last = (begin + it.r.units - 1) / share;
       return it;
     }
     left -= __shfl_sync(0xffffffffu, upto, 31);
@@ -300,9 +356,8 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
     Header h{};
     h.last = -1;
     if (it.pos < it.end && it.unit > 0) {  // the share begins inside a segment: others hold its beginning
-      const int begin = it.pos - it.unit;
-      h.first = begin / it.share;
-      h.last = (begin + it.r.units - 1) / it.share;
+      h.first = it.first;
+      h.last = it.last;
       h.row0 = it.tile * kRows;
       h.rows = min(kRows, it.r.fresh * p.group - h.row0);
       h.token0 = it.r.token0;

@@ -364,6 +364,18 @@ def test_attention_matches_oracle(lengths, new, heads, kvh, dim, page, dtype):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("requests,longest,new,heads,kvh,dim", [
+    (5, 800, 1, 64, 64, 64), (7, 2500, 3, 16, 2, 64), (33, 900, 1, 8, 2, 64), (64, 600, 2, 8, 2, 128), (60, 1100, 1, 8, 8, 64),
+    (65, 700, 1, 8, 4, 64), (2, 9000, 16, 64, 8, 64), (32, 1500, 4, 12, 1, 256)])
+def test_batches_that_are_cut_in_different_ways(requests, longest, new, heads, kvh, dim):
+    """Segments with CTAs of their own, equal shares across segments, and more requests than a warp holds."""
+    rng = np.random.default_rng(requests)
+    lengths = [longest, *(int(x) for x in rng.integers(0, longest, requests - 1))]
+    fresh = [min(n, int(x)) for n, x in zip(lengths, rng.integers(0, new + 1, requests))]
+    fresh[0] = new
+    test_attention_matches_oracle(lengths, fresh, heads, kvh, dim, 16, "bf16")
+
+
 @pytest.mark.parametrize("strong", [2.0 ** -12, 100.0, 3000.0])
 def test_attention_over_weak_and_strong_rows(strong):
     """V scales far from 1 move the weights' reference exponent; strong keys make the softmax one-hot."""

@@ -5,8 +5,9 @@
 // BF16, INT8 per-row and E2M1/FP16-per-32 weights with 16-byte rows: two launches.
 //   adapter_stream_kernel reads W and the tokens' A once, as one list of work: a block is 128 rows (8 warps x 16 rows) of W,
 //   or 8 groups of 16 rows of the tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or
-//   256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM, so any N and K
-//   and any number of adapters keep every SM reading to the end. A warp copies its units into a ring of its own (cp.async,
+//   256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM (a block into
+//   shares of its own where that costs little), so any N and K and any number of adapters keep every SM reading to the
+//   end. A warp copies its units into a ring of its own (cp.async,
 //   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this takes 31.3) and
 //   multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16 bytes of rows g and
 //   g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies in shared memory in
@@ -17,8 +18,9 @@
 //   y + t . B_a[n] with one rounding.
 // Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
 //
-// What bounds it: HBM while the units stream (142 MB in 21 us at M = 16, 14336 -> 4096, rank 64), around it launch, the
-// staging of x (1 to 2.5 us) and the join (3 us).
+// What bounds it: HBM while the units stream (142 MB in 21 us at M = 16, 14336 -> 4096, rank 64; 31.9 us in all), around
+// it launch, the staging of x (1 to 2.5 us) and the join (3 us). M = 1, 4096 -> 4096 BF16 7.5 us, M = 8, 4096 -> 14336
+// INT8 17.0.
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -138,6 +140,10 @@ constexpr int kAsRows = 16 * kAsWarps;   // rows of a block
 constexpr int kAsTokens = 16;            // tokens of a call's tile
 constexpr int kAsWindow = 32 * 1024;     // x in shared memory
 constexpr int kAsMinShare = 2;           // units of a share: fewer would only add records to join
+// Every block gets CTAs of its own where shares grow by at most so many units: a second piece stages x again and starts its
+// ring anew. M = 4, 1856 -> 1000 BF16 4.7 us (equal shares 6.2), M = 16, 4096 -> 14336 E2M1 27.3 (28.2), M = 8 INT8 17.0
+// (17.3); 8 units gain nothing more.
+constexpr int kAsSlack = 4;
 
 // Bytes of a row in a unit and units of a warp in flight, by the kind of W. Longer runs of a row are better for HBM, shorter
 // units even out short shares: M = 16, 14336 -> 4096 BF16 takes 31.3 us with 256-byte units and 33.4 with 128; M = 8,
@@ -172,6 +178,7 @@ struct StreamParams {
   int a_blocks, w_blocks;        // per tile of 16 tokens
   int a_units, w_units;          // units of a block
   int share, a_pieces, w_pieces; // units of a CTA; most shares that meet in a block
+  int a_parts, w_parts;          // CTAs of a block where none takes parts of two (w_parts = 0: equal shares)
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -450,14 +457,27 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
   const int tile = blockIdx.y, token0 = tile * kAsTokens;
   const unsigned ring = smem_addr(xs) + kAsWindow + warp * as_depth(KIND) * as_slot(KIND);
   const int a_total = p.a_blocks * p.a_units, total = a_total + p.w_blocks * p.w_units;
-  int pos = min(static_cast<long long>(blockIdx.x) * p.share, static_cast<long long>(total));
-  const int end = min(pos + p.share, total);
+  int pos = p.w_parts ? 0 : min(static_cast<long long>(blockIdx.x) * p.share, static_cast<long long>(total));
+  const int end = p.w_parts ? 1 : min(pos + p.share, total);
   bool first = true;
   while (pos < end) {
-    const bool is_a = pos < a_total;
-    const int units = is_a ? p.a_units : p.w_units, from = is_a ? 0 : a_total;
-    const int block = (pos - from) / units, u0 = pos - from - block * units, u1 = min(units, u0 + end - pos);
-    const int begin = from + block * units, piece = blockIdx.x - begin / p.share;
+    bool is_a;
+    int block, u0, u1, piece;
+    if (p.w_parts) {  // one piece
+      const int a_ctas = p.a_blocks * p.a_parts, cta = blockIdx.x;
+      is_a = cta < a_ctas;
+      const int parts = is_a ? p.a_parts : p.w_parts, units = is_a ? p.a_units : p.w_units, at = is_a ? cta : cta - a_ctas;
+      block = at / parts, piece = at - block * parts;
+      u0 = static_cast<int>(static_cast<long long>(piece) * units / parts);
+      u1 = static_cast<int>(static_cast<long long>(piece + 1) * units / parts);
+      pos = end;
+    } else {
+      is_a = pos < a_total;
+      const int units = is_a ? p.a_units : p.w_units, from = is_a ? 0 : a_total;
+      block = (pos - from) / units, u0 = pos - from - block * units, u1 = min(units, u0 + end - pos);
+      piece = blockIdx.x - (from + block * units) / p.share;
+      pos += u1 - u0;
+    }
     float sum[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -477,7 +497,8 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       const unsigned char* base = has ? reinterpret_cast<const unsigned char*>(
                                             p.a + (static_cast<long long>(id) * p.rank + 16 * rg) * p.k)
                                       : nullptr;
-      stream_piece<AD_BF16, NB, as_unit(KIND), as_depth(KIND)>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1, token0, xs, ring, top, sum, false);
+      stream_piece<AD_BF16, NB, as_unit(KIND), as_depth(KIND)>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1,
+                                                               token0, xs, ring, top, sum, false);
       if (has) {
         const int column = token - token0;
         float* to = p.a_part + ((static_cast<long long>(tile) * p.a_blocks + block) * p.a_pieces + piece) * kAsRows + 16 * warp;
@@ -491,8 +512,8 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       const int row0 = block * kAsRows + 16 * warp, rows = p.n - row0;
       const unsigned short* scales =
           KIND == AD_FP4 ? static_cast<const unsigned short*>(p.side) + static_cast<long long>(row0) * (p.k / 32) : nullptr;
-      stream_piece<KIND, NB, as_unit(KIND), as_depth(KIND)>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes, scales, rows, u0, u1, token0, xs,
-                             ring, top, sum, first);
+      stream_piece<KIND, NB, as_unit(KIND), as_depth(KIND)>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes,
+                                                            scales, rows, u0, u1, token0, xs, ring, top, sum, first);
       first = false;
       const int tokens = min(kAsTokens, p.m - token0);
       float* to = p.w_part + (((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces + piece) * kAsTokens) * kAsRows +
@@ -505,7 +526,6 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
           if (token < tokens) to[token * kAsRows + g + (e & 2 ? 8 : 0)] = sum[b][e];
         }
     }
-    pos += u1 - u0;
   }
 }
 
@@ -530,7 +550,7 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
   grid_launch_dependents();
   // The shares of the block, in order.
   const int begin = p.a_blocks * p.a_units + block * p.w_units;
-  const int pieces = (begin + p.w_units - 1) / p.share - begin / p.share + 1;
+  const int pieces = p.w_parts ? p.w_parts : (begin + p.w_units - 1) / p.share - begin / p.share + 1;
   const float* from = p.w_part + ((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces * kAsTokens + slot) * kAsRows + tid;
   float y = 0.0f;
   for (int q0 = 0; q0 < pieces; q0 += 8) {
@@ -543,7 +563,8 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
   }
   for (int r = tid; r < 8 * runs; r += kAsRows) {
     const int group = slot * p.groups + r / 16, ablock = group / kAsWarps;
-    const int abegin = ablock * p.a_units, apieces = (abegin + p.a_units - 1) / p.share - abegin / p.share + 1;
+    const int abegin = ablock * p.a_units;
+    const int apieces = p.w_parts ? p.a_parts : (abegin + p.a_units - 1) / p.share - abegin / p.share + 1;
     const float* src = p.a_part + (static_cast<long long>(tile) * p.a_blocks + ablock) * p.a_pieces * kAsRows +
                        16 * (group % kAsWarps) + r % 16;
     float t = 0.0f;
@@ -610,6 +631,15 @@ StreamPlan plan_stream(int kind, StreamParams& p, int places) {
   s.ctas = static_cast<int>((total + p.share - 1) / p.share);
   p.a_pieces = (p.a_units - 1) / p.share + 2;
   p.w_pieces = (p.w_units - 1) / p.share + 2;
+  p.a_parts = p.w_parts = 0;
+  for (int own = p.share; own <= p.share + kAsSlack; ++own) {
+    const int a_parts = (p.a_units + own - 1) / own, w_parts = (p.w_units + own - 1) / own;
+    const long long ctas = static_cast<long long>(p.a_blocks) * a_parts + static_cast<long long>(p.w_blocks) * w_parts;
+    if (ctas > places) continue;
+    p.a_parts = p.a_pieces = a_parts, p.w_parts = p.w_pieces = w_parts;
+    s.ctas = static_cast<int>(ctas);
+    break;
+  }
   s.a_part = static_cast<size_t>(s.tiles) * p.w_blocks * p.w_pieces * kAsTokens * kAsRows * 4;
   s.total = s.a_part + static_cast<size_t>(s.tiles) * p.a_blocks * p.a_pieces * kAsRows * 4;
   return s;

@@ -80,6 +80,13 @@ def test_matches_oracle(kind, m, n, k, rank, count, dtype):
     assert adapter_linear(rest[0], w, *rest[1:], output_dtype=dtype, out=out) is out and torch.equal(out, y)
 
 
+@pytest.mark.parametrize("kind,m,n,k,rank,count", [("bf16", 2, 20000, 128, 8, 2), ("int8", 9, 9000, 2048, 24, 12), ("fp4", 16, 4500, 1024, 8, 3),
+                                                   ("bf16", 20, 6000, 1000, 40, 5), ("int8", 1, 128, 16384, 16, 1)])
+def test_rows_cut_in_different_ways(kind, m, n, k, rank, count):
+    """More blocks of rows than there are CTAs, and few blocks over a long K."""
+    test_matches_oracle(kind, m, n, k, rank, count, torch.bfloat16)
+
+
 def test_rows_depend_on_their_own_adapter_alone(native):
     """All rows without one, all with the same one, mixed, and indices outside the stack (counted as none, reported)."""
     from klab_b200.adapters import adapter_linear

@@ -18,15 +18,16 @@
 //                 32 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
 //                 more MMA of the scales with the groups' sums of q in two FP16 terms, and starts the sum.
 //   softmax       in base 2 against a reference `ref` of the row that moves only when a score passes it by 2^14, so most
-//                 units need no rescale and no cross-lane maximum; sums in FP32.
-//   O^T += V^T P' A = 16 dims x 16 tokens of codes (FP16 subnormals), B = P' = p * (V scale of the token and group) in
-//                 FP16, below 2^15 with room under it for the tail (FP16 subnormals end 2^-34 under the row's largest
-//                 weight at scales near 1). For BF16 outputs p and the product are rounded to FP16 in turn (2^-11 relative
-//                 each at most: 3 * 10^-4 of the result in the mean, a fifth of BF16's own 1.7 * 10^-3); for FP16 outputs
-//                 the product is formed in FP32 and rounded once (both roundings would show beside FP16's 2 * 10^-4; it
-//                 costs 6 %). sum P' of each group comes from an MMA with ones, and -8 sum P' turns u into u - 8 at the
-//                 end, so u and 8 meet the same P' and a code of 8 stays an exact 0. (One MMA of the scales with p in place
-//                 of the four with ones saved 1.5 % and lost that.)
+//                 units need no rescale and no cross-lane maximum; weights and sums in FP32.
+//   O^T += V^T P' A = 16 dims x 16 tokens of codes (FP16 subnormals), B = P' = p * (V scale of the token and group), formed
+//                 in FP32 and rounded once to FP16 (2^-11 relative at most, for the tensor cores' sake). `ref` counts the
+//                 range of the V scales in (below 2^-7, below 2, or any): p can be 2^22 for weak rows and 2^-1 for strong
+//                 ones, and P' stays below 2^15 with room under it for the tail, 2^-34 to 2^-27 of the row's largest weight
+//                 where its scale is near its range's. (p rounded to FP16 first saves 3 % for BF16 outputs, adds as much
+//                 error again, and leaves FP16 where the scales of one row are far from another's.) sum P' of each group
+//                 comes from an MMA with ones, and -8 sum P' turns u into u - 8 at the end, so u and 8 meet the same P' and a
+//                 code of 8 stays an exact 0. (One MMA of the scales with p in place of the four with ones saved 1.5 % and
+//                 lost that.)
 // Scores beyond a row's last position are -inf before the softmax, and the scales of tokens beyond the request are zeroed,
 // so whatever the allocator left there (NaN scales included) has no part.
 //
@@ -68,9 +69,12 @@ constexpr int kUnitTokens = 2 * kKvBlock;
 // 1 x 2000 16.6 us whole and 7.7 cut.
 constexpr int kWholeUnits = 16;
 constexpr float kNegInf = -__builtin_huge_valf();
-// A row's weights are 2^(score - ref) with ref = (a score near the largest) - 10, moved when a score passes it by 2^14; V
-// scales below 2 then keep P' below 2^15.
+// A row's weights are 2^(score - ref) with ref = (a score near the largest) - 10 + e, moved when a score passes it by
+// 14 - e; V scales below 2^(e + 1) then keep P' below 2^15. e is that of the range of the scales a warp has met: FP16 patterns
+// say by their two highest exponent bits whether one is 2^-7 or more, and 2 or more.
 constexpr float kRefBelow = 10.0f, kMoveAt = 14.0f;
+constexpr float kWeakRange = -8.0f, kPlainRange = 0.0f, kStrongRange = 15.0f;
+constexpr unsigned kAboveWeak = 0x60006000u, kAbovePlain = 0x40004000u;
 
 // Of each CTA: where its share begins inside a segment (a tile of rows of a request), what the CTAs from `first` to `last`
 // of that segment left in scratch has to be joined.
@@ -121,18 +125,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ unsigned pack_h2(float lo, float hi) {
   unsigned r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-__device__ __forceinline__ unsigned mul_h2(unsigned a, unsigned b) {
-  unsigned r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
-__device__ __forceinline__ unsigned max_h2(unsigned a, unsigned b) {
-  unsigned r;
-  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -501,8 +493,9 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
       for (int i = 0; i < NG / 2; ++i) ones[i][e] = 0.0f;
     l[0] = l[1] = 0.0f;
     nref[0] = nref[1] = -kNegInf;
-    const int tv = kBf16 ? t : g >> 1;  // the token pair whose V scales this lane holds
-    int vshift = 0;                     // V scales are taken times 2^-vshift, which is below 2
+    const int tv = g >> 1;              // the token pair whose V scales this lane holds
+    float range = kWeakRange;           // e of the V scales
+    unsigned above = kAboveWeak;        // bits that scales of the range do not have
     unsigned ok = 0;            // blocks of the window being read that have a page
     bool live = true;
 
@@ -589,16 +582,7 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
         }
       }
 
-      // ---- does the reference still hold, and are the V scales below 2 (bit 14 of a positive FP16 says so)?
-      if (vshift) {
-        const unsigned by = static_cast<unsigned>((15 - vshift) << 10) * 0x10001u;  // 2^-vshift, vshift <= 15
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int G = 0; G < NG; ++G) sv[b][j][G] = mul_h2(sv[b][j][G], by);
-      }
+      // ---- does the reference still hold, and are the V scales in the range?
       unsigned any = 0u;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -609,38 +593,23 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) most = fmaxf(most, fmaxf(y[b][e], y[b][e + 1]));
-      if (__any_sync(0xffffffffu, most > kMoveAt || (any & 0x40004000u))) {
-        unsigned vtop = 0u;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int G = 0; G < NG; ++G) vtop = max_h2(vtop, max_h2(sv[b][0][G], sv[b][1][G]));
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) vtop = max_h2(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-        // v < 2^exponent; the scales become those below 2
-        const float v = fmaxf(lo_f32(vtop), hi_f32(vtop));
-        const int more = max(0, static_cast<int>(__float_as_uint(v) >> 23) - 126 - 1);
-        const float by_shift = __int_as_float((127 - more) << 23);
-        if (more) {
-          const unsigned by = static_cast<unsigned>((15 - more) << 10) * 0x10001u;
-          vshift += more;
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int G = 0; G < NG; ++G) sv[b][j][G] = mul_h2(sv[b][j][G], by);
-        }
+      if (__any_sync(0xffffffffu, most > kMoveAt - range || (any & above))) {
+        any = __reduce_or_sync(0xffffffffu, any);
+        const float before = range;
+        if (any & kAbovePlain)
+          range = kStrongRange, above = 0u;
+        else if (any & kAboveWeak)
+          range = fmaxf(range, kPlainRange), above &= kAbovePlain;
+        const float wider = range - before;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = fmaxf(fmaxf(x[0][e], x[0][e + 2]), fmaxf(x[1][e], x[1][e + 2])) * rs[e];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          const float was = -nref[e], now = fmaxf(top - kRefBelow, was);
+          const float was = -nref[e], now = fmaxf(top - kRefBelow + range, was + wider);
           if (was != kNegInf) {
-            float factor = exp2_fast(was - now);
+            const float factor = exp2_fast(was - now);
             l[e] *= factor;
-            factor *= by_shift;
 #pragma unroll
             for (int i = 0; i < 2 * NG; ++i) o[i][e] *= factor, o[i][e + 2] *= factor;
 #pragma unroll
@@ -660,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
       // ---- P, its sums, P' per group as B fragments (rows x tokens), O^T += V^T P'
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        unsigned pb[2], vw[2][NG];
+        unsigned vw[2][NG];
         float w[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -675,25 +644,13 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
         for (int e = 0; e < 4; ++e) w[e] = exp2_fast(y[b][e]);
         l[0] += w[0] + w[2];
         l[1] += w[1] + w[3];
-        if (kBf16) {
-          pb[0] = transpose8x8(pack_h2(w[0], w[1]));
-          pb[1] = transpose8x8(pack_h2(w[2], w[3]));
-        }
 #pragma unroll
         for (int G = 0; G < NG; ++G) {
           const unsigned a = vw[0][G], c = vw[1][G], ah = a >> 8, ch = c >> 8;
-          float s0 = 0.0f, s1 = 0.0f;
-          if (!kBf16) {
-            s0 = f16_to_f32(static_cast<unsigned short>(sv[b][0][G] >> (16 * (g & 1))));
-            s1 = f16_to_f32(static_cast<unsigned short>(sv[b][1][G] >> (16 * (g & 1))));
-          }
-          unsigned b0, b1;
-          if (kBf16) {
-            b0 = mul_h2(pb[0], sv[b][0][G]), b1 = mul_h2(pb[1], sv[b][1][G]);
-          } else {
-            b0 = transpose8x8(pack_h2(w[0] * s0, w[1] * s0));
-            b1 = transpose8x8(pack_h2(w[2] * s1, w[3] * s1));
-          }
+          const float s0 = f16_to_f32(static_cast<unsigned short>(sv[b][0][G] >> (16 * (g & 1))));
+          const float s1 = f16_to_f32(static_cast<unsigned short>(sv[b][1][G] >> (16 * (g & 1))));
+          const f2 p0 = mul2({w[0], w[1]}, {s0, s0}), p1 = mul2({w[2], w[3]}, {s1, s1});
+          const unsigned b0 = transpose8x8(pack_h2(p0.x, p0.y)), b1 = transpose8x8(pack_h2(p1.x, p1.y));
           mma_f16(o[2 * G], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, b0, b1,
                   o[2 * G]);
           mma_f16(o[2 * G + 1], ah & 0x000f000fu, ah & 0x00f000f0u, ch & 0x000f000fu, ch & 0x00f000f0u, b0, b1,
@@ -712,7 +669,6 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
     turn += count;
 
     // ---- the warps' sums to shared memory, joined there
-    const float unshift = __int_as_float((127 + vshift) << 23);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float sum = l[e];
@@ -724,12 +680,12 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
 #pragma unroll
       for (int G = 0; G < NG; ++G) {
         const float mass = ones[G / 2][G & 1 ? e + 2 : e];
-        const float eight = 8.0f * unshift * mass;
+        const float eight = 8.0f * mass;
         float4 v;
-        v.x = fmaf(o[2 * G][e], 16777216.0f * unshift, -eight);
-        v.y = fmaf(o[2 * G][e + 2], 1048576.0f * unshift, -eight);
-        v.z = fmaf(o[2 * G + 1][e], 16777216.0f * unshift, -eight);
-        v.w = fmaf(o[2 * G + 1][e + 2], 1048576.0f * unshift, -eight);
+        v.x = fmaf(o[2 * G][e], 16777216.0f, -eight);
+        v.y = fmaf(o[2 * G][e + 2], 1048576.0f, -eight);
+        v.z = fmaf(o[2 * G + 1][e], 16777216.0f, -eight);
+        v.w = fmaf(o[2 * G + 1][e + 2], 1048576.0f, -eight);
         *reinterpret_cast<float4*>(to + 32 * G + 4 * g) = v;
       }
     }

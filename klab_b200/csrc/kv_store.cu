@@ -63,16 +63,6 @@ __device__ __forceinline__ f2 widen2(unsigned w) {
   return kBf16 ? f2{bf16lo(w), bf16hi(w)} : f2{f16lo(w), f16hi(w)};
 }
 
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  unsigned long long ra, rb, rd;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(ra) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(rb) : "f"(b.x), "f"(b.y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(rd) : "l"(ra), "l"(rb));
-  f2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(rd));
-  return d;
-}
-
 template <bool kBf16>
 __device__ __forceinline__ void widen8(uint4 v, f2 (&x)[4]) {
   x[0] = widen2<kBf16>(v.x);

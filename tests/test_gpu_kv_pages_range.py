@@ -1,0 +1,83 @@
+"""Attention over 4-bit pages at the ends of its range: one huge value of V, weak values under a long tail."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_pages as ok
+from test_gpu_kv_pages import DT, f64, i32, native  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def one_request(k, v, page=16):
+    """Pages in order that hold these rows, and the table, lengths and starts of one token's attention over them."""
+    from klab_b200 import kv_pages
+
+    n, kvh, dim = k.shape
+    pages = -(-n // page)
+    buf = kv_pages.empty_pages(pages, kvh, page, dim)
+    buf.fill_(255)
+    kv_pages.store(k, v, buf, i32(np.arange(n)))
+    return buf, i32(np.arange(pages)[None]), i32([n]), i32([0, 1])
+
+
+@pytest.mark.parametrize("dtype,huge", [("bf16", 3e5), ("bf16", float("inf")), ("bf16", 2.0 ** 18), ("fp16", 6e4), ("fp16", 20.0)])
+@pytest.mark.parametrize("at", [5, 650], ids=["first", "late"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_one_huge_value_stays_in_its_group(dtype, huge, at, dim):
+    """A V scale up to the largest FP16 value, in the first tokens or behind many, against each group's own magnitude.
+
+    A weight times its V scale s is rounded to FP16 once, 2^-11 of itself or 2^-25 at worst. A warp's weights are taken so
+    that its largest is at least 2^(10 - e), with 2^e the end of the range of scales (2^-8, 2^0 or 2^15) that holds its own,
+    so the 2^-25 are at most 2^(e - 35) of the largest weight, and a value is s * (u - 8) with |u - 8| <= 8: over n tokens
+    8 n 2^(e - 35). The sums: an MMA adds its 16 products to the accumulator in single precision, in an order and with a
+    rounding that are not specified, so that beside one large term each of the n smaller ones may be cut, 2^-23 of the
+    accumulator a time, where `close` counts one for 16 rows of alike size: (n + 8) * 23 * 2^-23 M. It counts in the huge
+    value's own group alone. Everything else as in `close`.
+    """
+    from klab_b200 import kv_pages
+
+    n, heads, kvh = 700, 8, 2
+    gen = torch.Generator(device="cuda").manual_seed(at + dim)
+    k, v = (torch.randn(n, kvh, dim, generator=gen, device="cuda").to(DT[dtype]) for _ in range(2))
+    q = torch.randn(1, heads, dim, generator=gen, device="cuda").to(DT[dtype])
+    v[at, 0, 3] = huge
+    out = f64(kv_pages.attention(q, *one_request(k, v)))
+    (kc, ks), (vc, vs) = (ok.quantize(f64(x)) for x in (k, v))
+    kk, vv = ok.values(kc, ks), ok.values(vc, vs)
+    want, size = ok.attention(f64(q), kk, vv, 1, dim ** -0.5)
+    mass, _ = ok.attention(f64(q), kk, np.repeat(vs, 32, -1), 1, dim ** -0.5)
+    half = torch.finfo(DT[dtype]).eps / 2
+    qs = np.abs(f64(q)).reshape(1, kvh, -1, dim // 32, 32).sum(-1)
+    d = 92 * 2.0 ** -23 * dim ** -0.5 * np.einsum("nhgG,hG->nhg", qs, ks.max(0)).reshape(1, -1, 1)
+    tol = half * np.abs(want) + (1 + half) * ((2.0 ** -11 + 2.0 ** -13 + 2 * d) * size + 8 * n * 2.0 ** (15 - 35)
+                                             + (n + 8) * 23 * 2.0 ** -23 * mass)
+    assert np.isfinite(out).all()
+    err = np.abs(out - want) - tol
+    assert (err <= 0).all(), err.max()
+    # What no bound of the sums hides: the other groups still hold their own mean to a few per cent.
+    others = out[0, :, 32:]
+    assert np.abs(others - want[0, :, 32:]).max() <= 0.05 * np.abs(want[0, :, 32:]).max()
+
+
+def test_weak_values_keep_a_long_tail():
+    """V scales of 2^-20: a token that outweighs each of the others by 2^13.4, and the others' sum, which counts.
+
+    All rows behind the first are alike, so the answer has a closed form. Error: the weights' one rounding to FP16 (2^-11;
+    their range is the scales', so none of them is an FP16 subnormal: 2^(10 + 8 - 13.5 - 20) is above 2^-16, off by 2^-25 at
+    worst, 2^-9 of it), exp2 and the sums in FP32 (2^-13), half a step of BF16.
+    """
+    from klab_b200 import kv_pages
+
+    n, kvh, dim = 6000, 148, 64
+    k = torch.zeros(n, kvh, dim, device="cuda", dtype=torch.bfloat16)
+    v = torch.full((n, kvh, dim), 7 * 2.0 ** -20, device="cuda", dtype=torch.bfloat16)
+    k[0], v[0] = 1.0, 0.0
+    q = torch.ones(1, kvh, dim, device="cuda", dtype=torch.bfloat16)
+    kk = ok.values(*ok.quantize(np.ones((1, 32))))[0, 0]
+    scale = float(np.float32(np.log(2.0) * (14 - np.log2(1.5)) / (64 * kk)))
+    out = f64(kv_pages.attention(q, *one_request(k, v), scale=scale))
+    tail = (n - 1) * np.exp(-scale * 64 * kk)
+    want = 7 * 2.0 ** -20 * tail / (1 + tail)
+    assert np.abs(out / want - 1).max() <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -12

@@ -425,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int ef = max(static_cast<int>(__float_as_uint(top) >> 23), 15);
     const float up = __uint_as_float(static_cast<unsigned>(268 - ef) << 23);  // 2^(141 - ef): the maximum becomes < 2^15
-    const float mine_rs = p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 14) << 23) * 16777216.0f;
+    // At most the largest float: scores that far apart are one-hot at any factor of that size, and 0 stays 0.
+    const float mine_rs = fminf(p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 14) << 23) * 16777216.0f, 3.402823466e38f);
     float c0[NG][2];  // of rows 2 t, 2 t + 1
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
@@ -603,7 +604,8 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
         const float wider = range - before;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(fmaxf(x[0][e], x[0][e + 2]), fmaxf(x[1][e], x[1][e + 2])) * rs[e];
+          float top = fmaxf(fmaxf(x[0][e], x[0][e + 2]), fmaxf(x[1][e], x[1][e + 2]));
+          top = mul_rn(top, rs[e]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
           const float was = -nref[e], now = fmaxf(top - kRefBelow + range, was + wider);
@@ -620,8 +622,10 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int h = 0; h < 4; h += 2) {
-              const float v = x[b][e + h];
-              y[b][e + h] = v == kNegInf ? kNegInf : fmaf(v, rs[e], -now);
+              // Scores past 2^27 know the weight only to a power of two: the largest score's is in range here, where a
+              // fused product would leave the score's own rounding, and no weight passes the limit.
+              const float v = x[b][e + h], score = mul_rn(v, rs[e]) - now, limit = kMoveAt - range;
+              y[b][e + h] = v == kNegInf ? kNegInf : score > limit ? limit : score;
             }
         }
       }

@@ -1,11 +1,12 @@
-"""Attention over 4-bit pages at the ends of its range: one huge value of V, weak values under a long tail."""
+"""Attention over 4-bit pages at the ends of its range: one huge value of V, weak values under a long tail, and scores and
+scales near the largest floats."""
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import kv_pages as ok
-from test_gpu_kv_pages import DT, f64, i32, native  # noqa: F401
+from test_gpu_kv_pages import DT, close, f64, i32, native  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,29 @@ def test_weak_values_keep_a_long_tail():
     tail = (n - 1) * np.exp(-scale * 64 * kk)
     want = 7 * 2.0 ** -20 * tail / (1 + tail)
     assert np.abs(out / want - 1).max() <= 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11 + 2.0 ** -12
+
+
+@pytest.mark.parametrize("dtype,times,scale", [("bf16", 2.0 ** 28, None), ("bf16", 2.0 ** 100, None), ("bf16", 2.0 ** 122, None),
+                                               ("bf16", 1.0, 2.9e38), ("fp16", 1.0, 1e30), ("fp16", 2.0 ** 12, 2.0 ** 20),
+                                               ("bf16", 2.0 ** -120, 2.0 ** 100), ("bf16", 0.0, 2.9e38)])
+def test_far_scores_stay_finite(dtype, times, scale):
+    """Scores of 2^30 and far beyond: FP32 holds them to 2^-24 of themselves, so the first token of each row by far is the
+    whole result, rounded once; a query of zeros weighs all tokens alike."""
+    from klab_b200 import kv_pages
+
+    n, heads, kvh, dim = 300, 8, 2, 128
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.randn(n, kvh, dim, generator=gen, device="cuda").to(DT[dtype]) for _ in range(2))
+    q = (torch.randn(1, heads, dim, generator=gen, device="cuda") * times).to(DT[dtype])
+    out = kv_pages.attention(q, *one_request(k, v), scale=scale)
+    kk, vv = (ok.values(*ok.quantize(f64(x))) for x in (k, v))
+    s = np.einsum("hgd,phd->hgp", f64(q)[0].reshape(kvh, 4, dim), kk) * (dim ** -0.5 if scale is None else scale)
+    top = np.sort(s, -1)
+    if times:  # what decides is far above the rounding of a score
+        assert ((top[..., -1] - top[..., -2]) > 2.0 ** -18 * np.abs(s).max(-1)).all()
+    if times >= 1.0:
+        want = vv[s.argmax(-1), np.arange(kvh)[:, None]].reshape(heads, dim)
+        half = torch.finfo(DT[dtype]).eps / 2
+        assert (np.abs(f64(out)[0] - want) <= (half + 2.0 ** -10) * np.abs(want)).all()
+    else:
+        close(out, q, [0], [n], [1], k, v, dtype, scale=scale if times else 1.0)

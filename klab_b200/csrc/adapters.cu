@@ -11,9 +11,9 @@
 //   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this takes 31.3) and
 //   multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16 bytes of rows g and
 //   g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies in shared memory in
-//   fragment order. BF16 weights meet BF16 x; INT8 codes and E2M1 values are exact in FP16 and meet x in FP16 times a power
-//   of two of the (token, window), E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block
-//   goes to scratch in FP32.
+//   fragment order. Weights, INT8 codes and E2M1 values are exact in BF16 and meet x as it is, so every product is exact
+//   whatever else the row holds; E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block goes
+//   to scratch in FP32.
 //   adapter_join_kernel adds the shares of each block in order, forms t = c (x A^T) the same way, and writes
 //   y + t . B_a[n] with one rounding.
 // Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
@@ -151,8 +151,7 @@ constexpr int kAsSlack = 4;
 __host__ __device__ constexpr int as_unit(int kind) { return kind == AD_BF16 ? 256 : 128; }
 __host__ __device__ constexpr int as_depth(int kind) { return kind == AD_BF16 ? 2 : 3; }
 
-// A warp's ring in shared memory: units of 16 rows, 16-byte chunk c of row r at chunk c ^ 4 (r mod 2), so that the fragment
-// loads (rows g, four chunks each) meet no bank twice.
+// A warp's ring in shared memory: units of 16 rows.
 __host__ __device__ constexpr int as_slot(int kind) { return 16 * as_unit(kind); }
 __host__ __device__ constexpr int as_smem(int kind) { return kAsWindow + kAsWarps * as_depth(kind) * as_slot(kind); }
 
@@ -189,35 +188,23 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Four INT8 codes as two FP16 pairs, exact: 0x6400 | (code + 128) is 1152 + code.
+// Four INT8 codes as two BF16 pairs, exact: with the code's low 7 bits u and its sign s, 0x4300 | u is 128 + u and
+// 0x4300 | s << 7 is 128 + 128 s.
 __device__ __forceinline__ void i8_pairs(unsigned w, unsigned& lo, unsigned& hi) {
-  const unsigned u = w ^ 0x80808080u;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x64646464u, 0x4140)), "r"(0x64806480u));
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x64646464u, 0x4342)), "r"(0x64806480u));
+  const unsigned u = w & 0x7f7f7f7fu, s = w & 0x80808080u;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x43434343u, 0x4140)), "r"(__byte_perm(s, 0x43434343u, 0x4140)));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x43434343u, 0x4342)), "r"(__byte_perm(s, 0x43434343u, 0x4342)));
 }
 
-// Words (lane t, i) -> (lane i, t) among the four lanes of a row: lane t's 16 bytes are group t, and leave it with word t of
-// each group.
-__device__ __forceinline__ void transpose_quad(uint4& v, int t) {
-  const bool odd = t & 1, high = t & 2;
-  unsigned s0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v.z : v.w, 1);
-  if (odd)
-    v.x = s0, v.z = s1;
-  else
-    v.y = s0, v.w = s1;
-  s0 = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, 2), s1 = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, 2);
-  if (high)
-    v.x = s0, v.y = s1;
-  else
-    v.z = s0, v.w = s1;
+// E2M1 codes J and J + 4 of a word as a BF16 pair, exact: the code's two exponent bits and one mantissa bit at BF16's lowest
+// exponent bits and highest mantissa bit are the value times 2^-126, BF16 subnormal included.
+template <int J>
+__device__ __forceinline__ unsigned e2m1_pair(unsigned w) {
+  const unsigned size = (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6) & 0x01c001c0u;
+  const unsigned by = ((J == 3 ? w : w << (12 - 4 * J)) & 0x80008000u) ^ 0x7e807e80u;  // +- 2^126
+  unsigned d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(size), "r"(by));
+  return d;
 }
 
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there) {
@@ -230,7 +217,7 @@ __device__ __forceinline__ void copy16(unsigned dst, const void* src, bool there
 template <int KIND, int NB, int UNIT, int DEPTH>
 __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsigned char* base, long long row_bytes,
                                              const unsigned short* scales, int rows, int u0, int u1, int token0,
-                                             unsigned char* xs, unsigned ring, int* top, float (&sum)[NB][4], bool first) {
+                                             unsigned char* xs, unsigned ring, float (&sum)[NB][4], bool first) {
   constexpr int P = as_pieces(KIND), COLS = as_cols(KIND);
   constexpr int kUnitSteps = UNIT / 64, kSlot = 16 * UNIT;  // an MMA step takes 64 bytes of each row
   constexpr int kStepBytes = P * NB * 512;  // x of one step
@@ -241,7 +228,10 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
   constexpr int kRun = UNIT / 16, kRowsAtOnce = 32 / kRun;
   const int sub = lane / kRun, chunk = lane % kRun;
   const unsigned char* mine = base + sub * row_bytes + 16 * chunk;
-  const unsigned to0 = ring + sub * UNIT + ((chunk ^ ((sub & 1) << 2)) << 4);
+  // Chunk c of row r at c ^ 4 (r mod 2) for fragments of 16 bytes (rows g, four chunks each), at c ^ (r mod 8) for words of
+  // a chunk (rows g): neither meets a bank twice.
+  static_assert(KIND != AD_FP4 || kRowsAtOnce == 4, "row j + sub, j a multiple of 4: the chunk's bit 2 turns with j's");
+  const unsigned to0 = ring + sub * UNIT + ((KIND == AD_FP4 ? chunk ^ sub : chunk ^ ((sub & 1) << 2)) << 4);
   int slot = 0;
   auto copy = [&](int u) {  // unit u into the ring's next slot; nothing past the piece, the rows or a row's end
     const long long at = static_cast<long long>(u) * UNIT;
@@ -250,7 +240,7 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
 #pragma unroll
     for (int j = 0; j < 16; j += kRowsAtOnce) {
       const bool there = in && j + sub < rows;
-      copy16(to + j * UNIT, there ? static_cast<const void*>(mine + at + j * row_bytes) : p.x, there);
+      copy16((KIND == AD_FP4 ? to ^ ((j & 4) << 4) : to) + j * UNIT, there ? static_cast<const void*>(mine + at + j * row_bytes) : p.x, there);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
@@ -301,10 +291,8 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
   const int s_end = kUnitSteps * u1;
   for (int s0 = kUnitSteps * u0; s0 < s_end; s0 += kSteps) {
     const int steps = min(kSteps, s_end - s0);
-    // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t)
+    // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t) ..
     __syncthreads();  // the last window is read
-    if (KIND != AD_BF16 && tid < kAsTokens) top[tid] = 0;
-    if (KIND != AD_BF16) __syncthreads();
     const int pieces = steps * P * NB * 32;
     auto fetch = [&](int i) {
       const int ln = i & 31, piece = (i >> 5) / NB % P, s = (i >> 5) / (NB * P);
@@ -322,37 +310,13 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = i0 + j * kAsThreads;
-        if (i < pieces) {  // uniform in a warp
-          if constexpr (KIND != AD_BF16) {  // the largest exponent of the token in the window
-            const unsigned u[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-            unsigned most = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) most = __vmaxu2(most, (u[e] >> 7) & 0x00ff00ffu);
-            int ef = max(most & 0xffffu, most >> 16);
-            ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 1));
-            ef = max(ef, __shfl_xor_sync(0xffffffffu, ef, 2));
-            if ((tid & 3) == 0) atomicMax(top + (i >> 5) % NB * 8 + ((i & 31) >> 2), ef);
-          }
-          reinterpret_cast<uint4*>(xs)[i] = v[j];
-        }
+        if constexpr (KIND == AD_FP4)  // columns j and j + 4 in a word, as e2m1_pair gives the weights
+          v[j] = make_uint4(__byte_perm(v[j].x, v[j].z, 0x5410), __byte_perm(v[j].x, v[j].z, 0x7632),
+                            __byte_perm(v[j].y, v[j].w, 0x5410), __byte_perm(v[j].y, v[j].w, 0x7632));
+        if (i < pieces) reinterpret_cast<uint4*>(xs)[i] = v[j];
       }
     }
     __syncthreads();
-    if constexpr (KIND != AD_BF16) {  // BF16 -> FP16 times 2^(141 - ef): the largest lands below 2^15
-      for (int i = tid; i < pieces; i += kAsThreads) {
-        const uint4 v = reinterpret_cast<const uint4*>(xs)[i];
-        unsigned u[4] = {v.x, v.y, v.z, v.w};
-        const int ef = min(max(top[(i >> 5) % NB * 8 + ((i & 31) >> 2)], 15), 254);
-        const float by = __int_as_float((268 - ef) << 23);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float lo = bf16lo(u[e]) * by, hi = bf16hi(u[e]) * by;
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[e]) : "f"(hi), "f"(lo));
-        }
-        reinterpret_cast<uint4*>(xs)[i] = make_uint4(u[0], u[1], u[2], u[3]);
-      }
-      __syncthreads();
-    }
     // ---- the window's steps
     float acc[NB][4];
 #pragma unroll
@@ -368,8 +332,18 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
       uint4 v[kUnitSteps][2];
 #pragma unroll
       for (int j = 0; j < kUnitSteps; ++j) {
-        const unsigned c = ((4 * j + t) ^ ((g & 1) << 2)) << 4;
-        v[j][0] = lds128(from + c), v[j][1] = lds128(from + c + 8 * UNIT);
+        if constexpr (KIND == AD_FP4) {  // word t of the step's four groups
+          unsigned c[2][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned at = from + (((4 * j + i) ^ g) << 4) + 4 * t;
+            c[0][i] = lds32(at), c[1][i] = lds32(at + 8 * UNIT);
+          }
+          v[j][0] = make_uint4(c[0][0], c[0][1], c[0][2], c[0][3]), v[j][1] = make_uint4(c[1][0], c[1][1], c[1][2], c[1][3]);
+        } else {
+          const unsigned c = ((4 * j + t) ^ ((g & 1) << 2)) << 4;
+          v[j][0] = lds128(from + c), v[j][1] = lds128(from + c + 8 * UNIT);
+        }
       }
       uint2 now0[kHeld], now1[kHeld];
       if constexpr (KIND == AD_FP4) {
@@ -381,7 +355,7 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
       copy(unit + DEPTH);
 #pragma unroll
       for (int j = 0; j < kUnitSteps; ++j) {
-        uint4 v0 = v[j][0], v1 = v[j][1];
+        const uint4 v0 = v[j][0], v1 = v[j][1];
         const unsigned xat = at + j * kStepBytes;
         if constexpr (KIND == AD_BF16) {
 #pragma unroll
@@ -405,27 +379,23 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
             i8_pairs(c1[i], a[1], a[3]);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
-              mma_f16(acc[b], a, i & 1 ? xv[b][i >> 1].z : xv[b][i >> 1].x, i & 1 ? xv[b][i >> 1].w : xv[b][i >> 1].y);
+              mma_bf16(acc[b], a, i & 1 ? xv[b][i >> 1].z : xv[b][i >> 1].x, i & 1 ? xv[b][i >> 1].w : xv[b][i >> 1].y);
           }
         } else {
-          transpose_quad(v0, t);
-          transpose_quad(v1, t);
           const unsigned c0[4] = {v0.x, v0.y, v0.z, v0.w}, c1[4] = {v1.x, v1.y, v1.z, v1.w};
           const unsigned g0[2] = {now0[j].x, now0[j].y}, g1[2] = {now1[j].x, now1[j].y};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {  // group i of the step: columns 8 t .. 8 t + 7 of it
-            const unsigned a0[4] = {e2m1x2_to_f16x2(c0[i] & 0xffu), e2m1x2_to_f16x2(c1[i] & 0xffu),
-                                    e2m1x2_to_f16x2(c0[i] >> 8 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 8 & 0xffu)};
-            const unsigned a1[4] = {e2m1x2_to_f16x2(c0[i] >> 16 & 0xffu), e2m1x2_to_f16x2(c1[i] >> 16 & 0xffu),
-                                    e2m1x2_to_f16x2(c0[i] >> 24), e2m1x2_to_f16x2(c1[i] >> 24)};
+            const unsigned a0[4] = {e2m1_pair<0>(c0[i]), e2m1_pair<0>(c1[i]), e2m1_pair<1>(c0[i]), e2m1_pair<1>(c1[i])};
+            const unsigned a1[4] = {e2m1_pair<2>(c0[i]), e2m1_pair<2>(c1[i]), e2m1_pair<3>(c0[i]), e2m1_pair<3>(c1[i])};
             const float h0 = f16_to_f32(static_cast<unsigned short>(g0[i >> 1] >> (16 * (i & 1))));
             const float h1 = f16_to_f32(static_cast<unsigned short>(g1[i >> 1] >> (16 * (i & 1))));
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
               const uint4 xv = lds128(xat + (i * NB + b) * 512);
               float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              mma_f16(d, a0, xv.x, xv.y);
-              mma_f16(d, a1, xv.z, xv.w);
+              mma_bf16(d, a0, xv.x, xv.y);
+              mma_bf16(d, a1, xv.z, xv.w);
               acc[b][0] = fma_rn(d[0], h0, acc[b][0]), acc[b][1] = fma_rn(d[1], h0, acc[b][1]);
               acc[b][2] = fma_rn(d[2], h1, acc[b][2]), acc[b][3] = fma_rn(d[3], h1, acc[b][3]);
             }
@@ -436,14 +406,7 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (KIND == AD_BF16) {
-          sum[b][e] += acc[b][e];
-        } else {
-          const int ef = min(max(top[8 * b + 2 * t + (e & 1)], 15), 254);
-          sum[b][e] = fma_rn(acc[b][e], __int_as_float((ef - 14) << 23), sum[b][e]);
-        }
-      }
+      for (int e = 0; e < 4; ++e) sum[b][e] += acc[b][e];
   }
   asm volatile("cp.async.wait_all;" ::: "memory");  // what is left copied nothing
   __syncwarp();  // the ring is free for the next piece
@@ -452,7 +415,6 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
 template <int KIND, int NB>
 __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const StreamParams p) {
   extern __shared__ __align__(128) unsigned char xs[];
-  __shared__ int top[kAsTokens];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int tile = blockIdx.y, token0 = tile * kAsTokens;
   const unsigned ring = smem_addr(xs) + kAsWindow + warp * as_depth(KIND) * as_slot(KIND);
@@ -498,7 +460,7 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
                                             p.a + (static_cast<long long>(id) * p.rank + 16 * rg) * p.k)
                                       : nullptr;
       stream_piece<AD_BF16, NB, as_unit(KIND), as_depth(KIND)>(p, base, 2ll * p.k, nullptr, min(16, p.rank - 16 * rg), u0, u1,
-                                                               token0, xs, ring, top, sum, false);
+                                                               token0, xs, ring, sum, false);
       if (has) {
         const int column = token - token0;
         float* to = p.a_part + ((static_cast<long long>(tile) * p.a_blocks + block) * p.a_pieces + piece) * kAsRows + 16 * warp;
@@ -513,7 +475,7 @@ __global__ void __launch_bounds__(kAsThreads, 2) adapter_stream_kernel(const Str
       const unsigned short* scales =
           KIND == AD_FP4 ? static_cast<const unsigned short*>(p.side) + static_cast<long long>(row0) * (p.k / 32) : nullptr;
       stream_piece<KIND, NB, as_unit(KIND), as_depth(KIND)>(p, rows > 0 ? p.w + row0 * p.row_bytes : nullptr, p.row_bytes,
-                                                            scales, rows, u0, u1, token0, xs, ring, top, sum, first);
+                                                            scales, rows, u0, u1, token0, xs, ring, sum, first);
       first = false;
       const int tokens = min(kAsTokens, p.m - token0);
       float* to = p.w_part + (((static_cast<long long>(tile) * p.w_blocks + block) * p.w_pieces + piece) * kAsTokens) * kAsRows +

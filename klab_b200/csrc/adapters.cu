@@ -188,20 +188,25 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const unsigned (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Four INT8 codes as two BF16 pairs, exact: with the code's low 7 bits u and its sign s, 0x4300 | u is 128 + u and
-// 0x4300 | s << 7 is 128 + 128 s.
+// INT8 codes and E2M1 values are taken times 2^-24, which the join takes back: their scales, which bring a sum into range,
+// come after it, and without it |x| of 2^121 makes a sum of codes infinite whose result is not. (Products of |x| under 2^-102
+// then reach FP32's subnormals.)
+constexpr float kAsUp = 16777216.0f;
+
+// Four INT8 codes times 2^-24 as two BF16 pairs, exact: with the code's low 7 bits u and its sign s, 0x3700 | u is
+// (128 + u) 2^-24 and 0x3700 | s << 7 is (128 + 128 s) 2^-24.
 __device__ __forceinline__ void i8_pairs(unsigned w, unsigned& lo, unsigned& hi) {
   const unsigned u = w & 0x7f7f7f7fu, s = w & 0x80808080u;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x43434343u, 0x4140)), "r"(__byte_perm(s, 0x43434343u, 0x4140)));
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x43434343u, 0x4342)), "r"(__byte_perm(s, 0x43434343u, 0x4342)));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(__byte_perm(u, 0x37373737u, 0x4140)), "r"(__byte_perm(s, 0x37373737u, 0x4140)));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x37373737u, 0x4342)), "r"(__byte_perm(s, 0x37373737u, 0x4342)));
 }
 
-// E2M1 codes J and J + 4 of a word as a BF16 pair, exact: the code's two exponent bits and one mantissa bit at BF16's lowest
+// E2M1 values J and J + 4 of a word times 2^-24 as a BF16 pair, exact: the code's two exponent bits and one mantissa bit at BF16's lowest
 // exponent bits and highest mantissa bit are the value times 2^-126, BF16 subnormal included.
 template <int J>
 __device__ __forceinline__ unsigned e2m1_pair(unsigned w) {
   const unsigned size = (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6) & 0x01c001c0u;
-  const unsigned by = ((J == 3 ? w : w << (12 - 4 * J)) & 0x80008000u) ^ 0x7e807e80u;  // +- 2^126
+  const unsigned by = ((J == 3 ? w : w << (12 - 4 * J)) & 0x80008000u) ^ 0x72807280u;  // +- 2^102
   unsigned d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(size), "r"(by));
   return d;
@@ -507,7 +512,7 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
 #pragma unroll
   for (int r = 0; r < kHeld; ++r) held[r] = r < runs ? __ldg(b + r) : make_uint4(0u, 0u, 0u, 0u);
   const float c = has ? __ldg(p.c + id) : 0.0f;
-  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + min(row, p.n - 1)) : 1.0f;
+  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + min(row, p.n - 1)) * kAsUp : kAsUp;
   grid_dependency_wait();
   grid_launch_dependents();
   // The shares of the block, in order.
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
   }
   __syncthreads();
   if (row >= p.n) return;
-  if (KIND == AD_I8) y = mul_rn(y, scale);
+  if (KIND != AD_BF16) y = mul_rn(y, scale);
   if (has) {
     float s0 = 0.0f, s1 = 0.0f;
     auto dot = [&](uint4 w, int r) {

@@ -1,4 +1,4 @@
-"""Adapters beside the shared projection: values of x far apart."""
+"""Adapters beside the shared projection: values of x far apart and near the largest."""
 
 import pytest
 import torch
@@ -32,3 +32,17 @@ def test_a_far_value_of_x_leaves_the_others(kind, m, far):
         exact = f64(w.dequantize())
     assert not exact[:, 7].any() and not exact[:, 1500].any()
     close(adapter_linear(x, w, a, b, c, ids, output_dtype=torch.float32), exact, x, a, b, c, ids, torch.float32)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp4"])
+@pytest.mark.parametrize("m", [1, 16])
+@pytest.mark.parametrize("times", [2.0 ** 124, 2.0 ** 121, 2.0 ** 60, 2.0 ** -60])
+def test_x_near_the_ends_of_its_range(kind, m, times):
+    """Sums whose value is in range although those of the weights' codes would not be."""
+    from klab_b200.adapters import adapter_linear
+
+    w, exact, x, a, b, c, ids = case(kind, m, 200, 1024, 8, 2, seed=4)
+    x = x * times
+    y = adapter_linear(x, w, a, b, c, ids, output_dtype=torch.float32)
+    assert y.isfinite().all()
+    close(y.double() / times, exact, x.double() / times, a, b, c, ids, torch.float32)

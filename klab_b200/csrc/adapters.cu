@@ -16,7 +16,10 @@
 //   to scratch in FP32.
 //   adapter_join_kernel adds the shares of each block in order, forms t = c (x A^T) the same way, and writes
 //   y + t . B_a[n] with one rounding.
+//   More than 16 rows are tiles of 16 that read W again each, from L2 where it holds it (the projections alone do the same,
+//   and take longer: BF16 M = 128 1022 us against 126, INT8 173 against 131).
 // Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
+// Either form takes parts of the rows one behind the other where the FP32 sums of all would pass 64 MiB.
 //
 // What bounds it: HBM while the units stream (142 MB in 21 us at M = 16, 14336 -> 4096, rank 64; 31.9 us in all), around
 // it launch, the staging of x (1 to 2.5 us) and the join (3 us). M = 1, 4096 -> 4096 BF16 7.5 us, M = 8, 4096 -> 14336
@@ -144,6 +147,12 @@ constexpr int kAsMinShare = 2;           // units of a share: fewer would only a
 // ring anew. M = 4, 1856 -> 1000 BF16 4.7 us (equal shares 6.2), M = 16, 4096 -> 14336 E2M1 27.3 (28.2), M = 8 INT8 17.0
 // (17.3); 8 units gain nothing more.
 constexpr int kAsSlack = 4;
+// CTAs to a place from which on blocks are not cut: the last round is then short, and no sums are joined. 4096 -> 14336 BF16,
+// M = 64 67 us (with 1: 76), M = 128 126 (137); 4096 -> 4096 INT8, M = 1024 276 us (with 8: 333). Cut for one tile alone, as
+// tiles of 16 rows run one behind the other, M = 128 took 158 and M = 2048, 4096 -> 4096 880 (599 now).
+constexpr int kAsWaves = 4;
+// FP32 sums that one pair of launches leaves; calls of more rows are made of several, on the same scratch.
+constexpr size_t kAsScratch = 64ull << 20;
 
 // Bytes of a row in a unit and units of a warp in flight, by the kind of W. Longer runs of a row are better for HBM, shorter
 // units even out short shares: M = 16, 14336 -> 4096 BF16 takes 31.3 us with 256-byte units and 33.4 with 128; M = 8,
@@ -581,7 +590,8 @@ bool stream_kind(int wfmt, int* kind) {
   return false;
 }
 
-// Fills the shares of p (m, n, k, rank set) for `places` CTAs.
+// Fills the shares of p (m, n, k, rank set) for `places` CTAs, which the tiles of 16 tokens share. Blocks are cut while that
+// fills the machine; from kAsWaves CTAs to a place on each is a share of its own, and its tile's sums are kept once.
 StreamPlan plan_stream(int kind, StreamParams& p, int places) {
   StreamPlan s{};
   p.row_bytes = kind == AD_BF16 ? 2ll * p.k : kind == AD_I8 ? p.k : p.k / 2;
@@ -592,24 +602,58 @@ StreamPlan plan_stream(int kind, StreamParams& p, int places) {
   p.w_blocks = (p.n + kAsRows - 1) / kAsRows;
   p.a_units = static_cast<int>((2ll * p.k + as_unit(kind) - 1) / as_unit(kind));
   p.w_units = static_cast<int>((p.row_bytes + as_unit(kind) - 1) / as_unit(kind));
-  const long long total = static_cast<long long>(p.a_blocks) * p.a_units + static_cast<long long>(p.w_blocks) * p.w_units;
-  const long long share = (total + places - 1) / places;
-  p.share = static_cast<int>(share < kAsMinShare ? kAsMinShare : share);
-  s.ctas = static_cast<int>((total + p.share - 1) / p.share);
-  p.a_pieces = (p.a_units - 1) / p.share + 2;
-  p.w_pieces = (p.w_units - 1) / p.share + 2;
-  p.a_parts = p.w_parts = 0;
-  for (int own = p.share; own <= p.share + kAsSlack; ++own) {
-    const int a_parts = (p.a_units + own - 1) / own, w_parts = (p.w_units + own - 1) / own;
-    const long long ctas = static_cast<long long>(p.a_blocks) * a_parts + static_cast<long long>(p.w_blocks) * w_parts;
-    if (ctas > places) continue;
-    p.a_parts = p.a_pieces = a_parts, p.w_parts = p.w_pieces = w_parts;
-    s.ctas = static_cast<int>(ctas);
-    break;
+  const long long blocks = static_cast<long long>(p.a_blocks) + p.w_blocks;
+  if (blocks * s.tiles >= static_cast<long long>(kAsWaves) * places) {
+    p.a_parts = p.w_parts = p.a_pieces = p.w_pieces = 1;
+    s.ctas = static_cast<int>(blocks);
+  } else {
+    const int here = places > s.tiles ? places / s.tiles : 1;
+    const long long total = static_cast<long long>(p.a_blocks) * p.a_units + static_cast<long long>(p.w_blocks) * p.w_units;
+    const long long share = (total + here - 1) / here;
+    p.share = static_cast<int>(share < kAsMinShare ? kAsMinShare : share);
+    s.ctas = static_cast<int>((total + p.share - 1) / p.share);
+    p.a_pieces = (p.a_units - 1) / p.share + 2;
+    p.w_pieces = (p.w_units - 1) / p.share + 2;
+    p.a_parts = p.w_parts = 0;
+    for (int own = p.share; own <= p.share + kAsSlack; ++own) {
+      const int a_parts = (p.a_units + own - 1) / own, w_parts = (p.w_units + own - 1) / own;
+      const long long ctas = static_cast<long long>(p.a_blocks) * a_parts + static_cast<long long>(p.w_blocks) * w_parts;
+      if (ctas > here) continue;
+      p.a_parts = p.a_pieces = a_parts, p.w_parts = p.w_pieces = w_parts;
+      s.ctas = static_cast<int>(ctas);
+      break;
+    }
   }
   s.a_part = static_cast<size_t>(s.tiles) * p.w_blocks * p.w_pieces * kAsTokens * kAsRows * 4;
   s.total = s.a_part + static_cast<size_t>(s.tiles) * p.a_blocks * p.a_pieces * kAsRows * 4;
   return s;
+}
+
+// Rows of x that one pair of launches takes, a whole number of tiles: all, or as many as leave their FP32 sums in kAsScratch
+// bytes (one tile at least).
+int stream_rows(int kind, int m, int n, int k, int rank, int places) {
+  StreamParams p{};
+  p.m = m, p.n = n, p.k = k, p.rank = rank;
+  const StreamPlan s = plan_stream(kind, p, places);
+  if (s.total <= kAsScratch) return m;
+  const size_t tile = (static_cast<size_t>(p.w_blocks) * kAsTokens + p.a_blocks) * kAsRows * 4;
+  const size_t tiles = tile < kAsScratch ? kAsScratch / tile : 1;
+  return static_cast<long long>(tiles) * kAsTokens < m ? static_cast<int>(tiles) * kAsTokens : m;
+}
+
+// The same for the form of three launches, whose scratch holds t and the projection in FP32. Every part has more than 16 rows
+// (or is the whole call), so that the projection asks for no more workspace than for all rows.
+int plain_rows(int m, int n, int rank) {
+  const size_t row = (static_cast<size_t>(n) + rank) * 4, rows = kAsScratch / row / kAsTokens * kAsTokens;
+  const int most = rows > 2 * kAsTokens ? static_cast<int>(rows < 65536 ? rows : 65536) : 2 * kAsTokens;
+  return m - most > kAsTokens ? most : m;
+}
+
+// Bytes of t, and of t and the projection, for up to `rows` rows of the call and the few behind the last part.
+size_t plain_t(int rows, int rank) { return (static_cast<size_t>(rows) * rank * 4 + 127) / 128 * 128; }
+size_t plain_scratch(int m, int n, int rank) {
+  const int rows = plain_rows(m, n, rank), held = rows < m ? rows + kAsTokens : m;
+  return plain_t(held, rank) + static_cast<size_t>(held) * n * 4;
 }
 
 template <typename Kernel>
@@ -682,15 +726,21 @@ extern "C" {
 KLAB_API long long klab_adapter_scratch(int wfmt, int m, int n, int k, int rank) {
   using namespace klab;
   if (m <= 0 || n <= 0 || k <= 0 || rank <= 0) return KLAB_E_INVALID;
-  const long long plain = (static_cast<long long>(m) * rank * 4 + 127) / 128 * 128 + static_cast<long long>(m) * n * 4;
+  size_t need = plain_scratch(m, n, rank);  // streamed formats with rows off 16-byte boundaries too
   int kind = 0, sms = 0;
-  if (!stream_kind(wfmt, &kind)) return plain;
-  const int rc = sm_count(&sms);
-  if (rc) return rc < 0 ? rc : -rc;
-  StreamParams p{};
-  p.m = m, p.n = n, p.k = k, p.rank = rank;
-  const long long shares = static_cast<long long>(plan_stream(kind, p, 2 * sms).total);
-  return shares > plain ? shares : plain;  // rows that are not 16-byte aligned take the plain form
+  if (stream_kind(wfmt, &kind)) {
+    const int rc = sm_count(&sms);
+    if (rc) return rc < 0 ? rc : -rc;
+    const int rows = stream_rows(kind, m, n, k, rank, 2 * sms);
+    for (const int part : {rows, m % rows}) {
+      if (!part) continue;
+      StreamParams p{};
+      p.m = part, p.n = n, p.k = k, p.rank = rank;
+      const size_t total = plan_stream(kind, p, 2 * sms).total;
+      if (total > need) need = total;
+    }
+  }
+  return static_cast<long long>(need);
 }
 
 KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const void* aux, const void* a, const void* b,
@@ -709,64 +759,79 @@ KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const v
                         reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(scratch);
   if (mis & 15) return KLAB_E_ALIGN;
   if (scratch_bytes < klab_adapter_scratch(wfmt, m, n, k, rank)) return KLAB_E_INVALID;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int out_bytes = out_dtype == KLAB_DT_F32 ? 4 : 2;
   int kind = 0;
   if (stream_kind(wfmt, &kind)) {
-    StreamParams q{};
-    q.m = m, q.n = n, q.k = k, q.rank = rank;
     int sms = 0;
     const int rc = sm_count(&sms);
     if (rc) return rc;
-    const StreamPlan plan = plan_stream(kind, q, 2 * sms);
+    const int rows = stream_rows(kind, m, n, k, rank, 2 * sms);
+    StreamParams q{};
+    q.m = rows, q.n = n, q.k = k, q.rank = rank;
+    plan_stream(kind, q, 2 * sms);
     if ((reinterpret_cast<uintptr_t>(w) & 15) == 0 && q.row_bytes % 16 == 0 &&
         static_cast<long long>(q.a_blocks) * q.a_units + static_cast<long long>(q.w_blocks) * q.w_units < INT_MAX) {
       if (kind != AD_BF16 && !aux) return KLAB_E_INVALID;
       if (kind == AD_FP4 && k % 32) return KLAB_E_SHAPE;
-      q.x = static_cast<const unsigned short*>(x);
       q.w = static_cast<const unsigned char*>(w);
       q.side = aux;
       q.a = static_cast<const unsigned short*>(a);
       q.b = static_cast<const unsigned short*>(b);
       q.c = c;
-      q.ids = ids;
       q.w_part = static_cast<float*>(scratch);
-      q.a_part = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + plan.a_part);
-      q.out = out;
       q.status = device_status_address();
       q.adapters = adapters;
       q.ldo = n;
       q.out_f32 = out_dtype == KLAB_DT_F32;
-      const cudaStream_t s = static_cast<cudaStream_t>(stream);
-      const bool one = m <= 8;
-      if (kind == AD_BF16) return one ? run_stream<AD_BF16, 1>(q, plan, s) : run_stream<AD_BF16, 2>(q, plan, s);
-      if (kind == AD_I8) return one ? run_stream<AD_I8, 1>(q, plan, s) : run_stream<AD_I8, 2>(q, plan, s);
-      return one ? run_stream<AD_FP4, 1>(q, plan, s) : run_stream<AD_FP4, 2>(q, plan, s);
+      for (int m0 = 0; m0 < m; m0 += rows) {
+        q.m = m - m0 < rows ? m - m0 : rows;
+        const StreamPlan plan = plan_stream(kind, q, 2 * sms);
+        q.a_part = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + plan.a_part);
+        q.x = static_cast<const unsigned short*>(x) + static_cast<long long>(m0) * k;
+        q.ids = ids + m0;
+        q.out = static_cast<unsigned char*>(out) + static_cast<long long>(m0) * n * out_bytes;
+        const bool one = q.m <= 8;
+        int rc;
+        if (kind == AD_BF16)
+          rc = one ? run_stream<AD_BF16, 1>(q, plan, s) : run_stream<AD_BF16, 2>(q, plan, s);
+        else if (kind == AD_I8)
+          rc = one ? run_stream<AD_I8, 1>(q, plan, s) : run_stream<AD_I8, 2>(q, plan, s);
+        else
+          rc = one ? run_stream<AD_FP4, 1>(q, plan, s) : run_stream<AD_FP4, 2>(q, plan, s);
+        if (rc) return rc;
+      }
+      return 0;
     }
   }
   AdapterParams p{};
-  p.x = static_cast<const unsigned short*>(x);
   p.a = static_cast<const unsigned short*>(a);
   p.b = static_cast<const unsigned short*>(b);
   p.c = c;
-  p.ids = ids;
-  p.t = static_cast<float*>(scratch);
-  float* y0 = p.t + (static_cast<long long>(m) * rank * 4 + 127) / 128 * 32;
-  p.y0 = y0;
-  p.out = out;
   p.status = device_status_address();
-  p.m = m;
   p.n = n;
   p.k = k;
   p.rank = rank;
   p.adapters = adapters;
   p.ldo = n;
   p.out_f32 = out_dtype == KLAB_DT_F32;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc = launch_adapter(shrink_kernel, dim3(rank / kRanks, m), p, s);
-  if (rc) return rc;
-  rc = klab_gemv(wfmt, KLAB_DT_BF16, x, k, w, aux, nullptr, y0, n, KLAB_DT_F32, m, n, k, workspace, workspace_bytes,
-                 stream);
-  if (rc) return rc;
-  return launch_adapter(expand_kernel, dim3((n + kAdThreads - 1) / kAdThreads, m), p, s);
+  p.t = static_cast<float*>(scratch);
+  const int part = plain_rows(m, n, rank);
+  for (int m0 = 0; m0 < m; m0 += p.m) {
+    p.m = m - m0 - part > kAsTokens ? part : m - m0;
+    float* y0 = p.t + plain_t(p.m, rank) / 4;
+    p.y0 = y0;
+    p.x = static_cast<const unsigned short*>(x) + static_cast<long long>(m0) * k;
+    p.ids = ids + m0;
+    p.out = static_cast<unsigned char*>(out) + static_cast<long long>(m0) * n * out_bytes;
+    int rc = launch_adapter(shrink_kernel, dim3(rank / kRanks, p.m), p, s);
+    if (rc) return rc;
+    rc = klab_gemv(wfmt, KLAB_DT_BF16, p.x, k, w, aux, nullptr, y0, n, KLAB_DT_F32, p.m, n, k, workspace, workspace_bytes, stream);
+    if (rc) return rc;
+    rc = launch_adapter(expand_kernel, dim3((n + kAdThreads - 1) / kAdThreads, p.m), p, s);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"

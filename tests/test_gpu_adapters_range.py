@@ -1,4 +1,5 @@
-"""Adapters beside the shared projection: values of x far apart and near the largest."""
+"""Adapters beside the shared projection: values of x far apart and near the largest, and
+many rows."""
 
 import pytest
 import torch
@@ -46,3 +47,24 @@ def test_x_near_the_ends_of_its_range(kind, m, times):
     y = adapter_linear(x, w, a, b, c, ids, output_dtype=torch.float32)
     assert y.isfinite().all()
     close(y.double() / times, exact, x.double() / times, a, b, c, ids, torch.float32)
+
+
+# Rows around and above a tile of 16; 2100 rows of 9000 outputs are two parts in either form.
+@pytest.mark.parametrize("kind,m,n,k,rank", [("bf16", 17, 300, 512, 16), ("int8", 129, 1000, 1024, 8), ("fp4", 129, 200, 2048, 24),
+                                             ("bf16", 2048, 520, 256, 16), ("bf16", 2100, 9000, 128, 8), ("int8", 2100, 9000, 128, 8),
+                                             ("fp4", 2100, 9000, 128, 8), ("coded", 2100, 9000, 128, 8), ("int8_64", 1870, 9000, 64, 8)])
+def test_many_rows(kind, m, n, k, rank):
+    from klab_b200.adapters import adapter_linear
+
+    w, exact, *rest = case(kind, m, n, k, rank, 5)
+    close(adapter_linear(rest[0], w, *rest[1:]), exact, *rest, torch.bfloat16)
+
+
+def test_scratch_stays_small(native):  # noqa: F811
+    """FP32 sums of 64 MiB at a time, whatever the number of rows."""
+    scratch = native.lib().klab_adapter_scratch
+    for wfmt in (native.W_BF16, native.W_I8_ROW, native.W_FP4_G32H, native.W_CBF16, native.W_I8_G64):
+        for m in (1, 16, 17, 500, 2048, 65535):
+            for n, k in ((14336, 4096), (4096, 14336), (100, 131072)):
+                for rank in (8, 256):
+                    assert 0 < scratch(wfmt, m, n, k, rank) <= 2 ** 26 + 2 ** 22, (wfmt, m, n, k, rank)

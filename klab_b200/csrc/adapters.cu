@@ -79,10 +79,11 @@ __global__ void __launch_bounds__(kAdThreads) shrink_kernel(const AdapterParams 
   const int chunks = p.k / 8;
 #pragma unroll 2
   for (int i = threadIdx.x; i < chunks; i += kAdThreads) {
-    const uint4 xv = __ldg(x + i);
+    // Not by read-only loads: this kernel may already be here while the launch before writes what it reads.
+    const uint4 xv = __ldcg(x + i);
     uint4 av[kRanks];
 #pragma unroll
-    for (int j = 0; j < kRanks; ++j) av[j] = ldg128_stream(a[j] + i);
+    for (int j = 0; j < kRanks; ++j) av[j] = __ldcg(a[j] + i);
 #pragma unroll
     for (int j = 0; j < kRanks; ++j) fma8(xv, av[j], s0[j], s1[j]);
   }
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kAdThreads) expand_kernel(const AdapterParams 
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll 4
     for (int j = 0; j < p.rank / 8; ++j) {
-      const uint4 w = __ldg(b + j);
+      const uint4 w = __ldcg(b + j);
       const float* tj = t + 8 * j;
       s0 = fma_rn(tj[0], bf16lo(w.x), s0), s1 = fma_rn(tj[1], bf16hi(w.x), s1);
       s0 = fma_rn(tj[2], bf16lo(w.y), s0), s1 = fma_rn(tj[3], bf16hi(w.y), s1);
@@ -273,15 +274,15 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
         const int i0 = 4 * (u * kUnitSteps + j);
         next0[j] = next1[j] = make_uint2(0u, 0u);
         if (scales_vec) {
-          if (u < u1 && i0 < srow && has0) next0[j] = __ldg(reinterpret_cast<const uint2*>(q0 + i0));
-          if (u < u1 && i0 < srow && has1) next1[j] = __ldg(reinterpret_cast<const uint2*>(q1 + i0));
+          if (u < u1 && i0 < srow && has0) next0[j] = __ldcg(reinterpret_cast<const uint2*>(q0 + i0));
+          if (u < u1 && i0 < srow && has1) next1[j] = __ldcg(reinterpret_cast<const uint2*>(q1 + i0));
         } else {
           unsigned short v[8] = {};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (u < u1 && i0 + i < srow) {
-              if (has0) v[i] = __ldg(q0 + i0 + i);
-              if (has1) v[4 + i] = __ldg(q1 + i0 + i);
+              if (has0) v[i] = __ldcg(q0 + i0 + i);
+              if (has1) v[4 + i] = __ldcg(q1 + i0 + i);
             }
           next0[j] = make_uint2(v[0] | static_cast<unsigned>(v[1]) << 16, v[2] | static_cast<unsigned>(v[3]) << 16);
           next1[j] = make_uint2(v[4] | static_cast<unsigned>(v[5]) << 16, v[6] | static_cast<unsigned>(v[7]) << 16);
@@ -519,9 +520,9 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
   const int runs = has ? p.rank / 8 : 0;
   uint4 held[kHeld];
 #pragma unroll
-  for (int r = 0; r < kHeld; ++r) held[r] = r < runs ? __ldg(b + r) : make_uint4(0u, 0u, 0u, 0u);
-  const float c = has ? __ldg(p.c + id) : 0.0f;
-  const float scale = KIND == AD_I8 ? __ldg(static_cast<const float*>(p.side) + min(row, p.n - 1)) * kAsUp : kAsUp;
+  for (int r = 0; r < kHeld; ++r) held[r] = r < runs ? __ldcg(b + r) : make_uint4(0u, 0u, 0u, 0u);
+  const float c = has ? __ldcg(p.c + id) : 0.0f;
+  const float scale = KIND == AD_I8 ? __ldcg(static_cast<const float*>(p.side) + min(row, p.n - 1)) * kAsUp : kAsUp;
   grid_dependency_wait();
   grid_launch_dependents();
   // The shares of the block, in order.
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(kAsRows) adapter_join_kernel(const StreamParam
 #pragma unroll
     for (int r = 0; r < kHeld; ++r)
       if (r < runs) dot(held[r], r);
-    for (int r = kHeld; r < runs; ++r) dot(__ldg(b + r), r);
+    for (int r = kHeld; r < runs; ++r) dot(__ldcg(b + r), r);
     y = add_rn(y, add_rn(s0, s1));
   }
   const long long at = static_cast<long long>(token) * p.ldo + row;

@@ -1,5 +1,5 @@
-"""Adapters beside the shared projection: values of x far apart and near the largest, and
-many rows."""
+"""Adapters beside the shared projection: values of x far apart and near the largest, many
+rows, and operands that the launch before wrote."""
 
 import pytest
 import torch
@@ -68,3 +68,48 @@ def test_scratch_stays_small(native):  # noqa: F811
             for n, k in ((14336, 4096), (4096, 14336), (100, 131072)):
                 for rank in (8, 256):
                     assert 0 < scratch(wfmt, m, n, k, rank) <= 2 ** 26 + 2 ** 22, (wfmt, m, n, k, rank)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("kind", ["coded", "int8_64", "int8", "fp4", "bf16"])
+def test_operands_that_the_launch_before_wrote(kind, captured):
+    """x, A, B, the adapters' scales, the ids and the weights' own scales come out of the launches right before the call: each
+    in turn is the last one written."""
+    from klab_b200.adapters import adapter_linear
+
+    w0, _, x0, a0, b0, c0, ids0 = case("bf16", 12, 1024, 512, 16, 3)
+    w, _, x, a, b, c, ids = case(kind, 12, 640, 1024, 16, 3, seed=1)
+    side = w.scales if kind in ("int8_64", "int8", "fp4") else c
+    held = {"a": a, "b": b, "c": c, "ids": ids, "side": side}
+    first = {k: t.clone() for k, t in held.items()}
+    ways = [lambda v: v, lambda v: v.flip(0).contiguous()]
+    sets = [{k: f(t) for k, t in first.items()} for f in ways]
+    xs = [f(x0) for f in ways]
+
+    def one(i, last):
+        for k in (*(k for k in held if k != last), *((last,) if last in held else ())):
+            held[k].copy_(sets[i][k])
+        if last == "x":
+            return adapter_linear(adapter_linear(xs[i], w0, a0, b0, c0, ids0, out=y), w, a, b, c, ids)
+        return adapter_linear(ys[i], w, a, b, c, ids)
+
+    y = torch.empty(12, 1024, device="cuda", dtype=torch.bfloat16)
+    ys = [adapter_linear(v, w0, a0, b0, c0, ids0) for v in xs]
+    want = []
+    for i in (0, 1):
+        for k, t in held.items():
+            t.copy_(sets[i][k])
+        torch.cuda.synchronize()
+        want.append(adapter_linear(ys[i], w, a, b, c, ids))
+    assert not torch.equal(*want)
+    order = [(i % 2, last) for i, last in enumerate(("x", "a", "b", "c", "ids", "side", "x") * 4)]
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = [one(*o) for o in order]
+        for _ in range(3):
+            g.replay()
+    else:
+        got = [one(*o) for o in order]
+    for v, (i, last) in zip(got, order):
+        assert torch.equal(v, want[i]), (i, last)

@@ -139,6 +139,8 @@ PyObject* guarded(F f) {
     return f();
   } catch (const Failed& e) {
     return PyLong_FromLong(e.code);  // the wrapper raises it
+  } catch (const c10::OutOfMemoryError&) {
+    return none();  // nothing was launched: the wrapper allocates, and raises torch's own error where it cannot
   } catch (const std::exception& e) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;

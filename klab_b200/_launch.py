@@ -4,7 +4,8 @@ A decode step makes several of these calls per layer, so their host time is the 
 calls go through the CPython module built from csrc/torch_binding.cpp (`fast`, loaded with the first device), which checks,
 allocates and launches in a few microseconds; whatever it answers None to comes back to the Python wrappers, which raise or
 launch through ctypes (`launch`): torch's current stream, the device switched only when it is not the current one, and the
-caching allocator told which stream used the tensors (_native.record).
+caching allocator told which stream used the tensors (_native.record). Where the binding was not built (no headers of torch
+or Python), every call goes that way, 10 to 16 us of host time slower.
 """
 
 from __future__ import annotations
@@ -13,6 +14,7 @@ import ctypes as ct
 import importlib.machinery
 import importlib.util
 import threading
+import warnings
 
 import torch
 
@@ -54,10 +56,13 @@ def ready(device):
         get_module(device)
         global fast
         with _lock:
-            module = fast or load_binding()
-            if index < 64:
-                module.mark_ready(index)
-            fast = module
+            if fast is None and BINDING.exists():
+                fast = load_binding()
+            if fast is None:
+                if not _ready:
+                    warnings.warn(f"{BINDING.name} is not built: batched operators launch through ctypes", RuntimeWarning, stacklevel=3)
+            elif index < 64:
+                fast.mark_ready(index)
             _ready.add(index)
     return index
 

@@ -110,24 +110,34 @@ def build(clean: bool = False, verbose: bool = False, out_dir: Path | None = Non
         ALIAS.unlink()
     ALIAS.symlink_to(LIBRARY.name)
     if out_dir is None:
-        build_binding()
         build_launcher()
+        build_binding()
     return LIBRARY
 
 
-def build_binding() -> Path:
-    """klab_torch.so from csrc/torch_binding.cpp (g++, torch's headers); rebuilt when torch's version changes."""
-    import torch
+def build_binding() -> Path | None:
+    """klab_torch.so from csrc/torch_binding.cpp (g++, torch's headers); rebuilt when torch's version changes. None, and no
+    binding, where the headers or the compiler are missing: the C library does not need it, and the batched operators take
+    their slower host path (_launch)."""
+    try:
+        import torch
+    except ImportError:
+        return _no_binding(["torch"])
 
     source, stamp = CSRC / "torch_binding.cpp", OBJ / "klab_torch.version"
     version = f"{torch.__version__} {sys.version}"
     if _stale(BINDING, [source, *_headers()]) or not stamp.exists() or stamp.read_text() != version:
         root = Path(torch.__file__).resolve().parent
         cuda = Path(nvcc()).resolve().parents[1]
-        cxx = shutil.which(os.environ.get("CXX", "g++")) or "g++"
+        python = Path(sysconfig.get_paths()["include"])
+        cxx = shutil.which(os.environ.get("CXX", "g++"))
+        needed = (python / "Python.h", root / "include/ATen/ATen.h", root / "include/torch/csrc/autograd/python_variable.h",
+                  cuda / "include/cuda_runtime.h")
+        missing = [str(h) for h in needed if not h.exists()] + ([] if cxx else ["g++"])
+        if missing:
+            return _no_binding(missing)
         tmp = BINDING.with_suffix(".new")
-        includes = [INCLUDE, root / "include", root / "include/torch/csrc/api/include", cuda / "include",
-                    sysconfig.get_paths()["include"]]
+        includes = [INCLUDE, root / "include", root / "include/torch/csrc/api/include", cuda / "include", python]
         _run([cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{i}" for i in includes],
               str(source), "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
@@ -135,6 +145,12 @@ def build_binding() -> Path:
         tmp.replace(BINDING)
         stamp.write_text(version)
     return BINDING
+
+
+def _no_binding(missing) -> None:
+    """Takes away a binding that does not fit this torch any more and says why there is none."""
+    BINDING.unlink(missing_ok=True)
+    print(f"{BINDING.name} not built, missing: {', '.join(missing)}", file=sys.stderr)
 
 
 def build_launcher() -> Path:

@@ -1,6 +1,8 @@
-"""Host side of the batched operators without a GPU: sizes of scratch."""
+"""Host side of the batched operators without a GPU: sizes of scratch, and a build where the binding's headers are missing."""
 
-from klab_b200 import _native
+import sysconfig
+
+from klab_b200 import _native, build
 
 
 def test_plain_scratch_stays_small():
@@ -11,3 +13,18 @@ def test_plain_scratch_stays_small():
             assert 4 * min(m, 1024) * 14336 < scratch(wfmt, m, 14336, 4096, 16) <= 2 ** 26 + 2 ** 21
         # Rows that are each past a part's size: two tiles and the rest of a third.
         assert scratch(wfmt, 100, 2 ** 24, 64, 8) == 48 * 4 * (2 ** 24 + 8)
+
+
+def test_build_without_python_headers(tmp_path, monkeypatch, capsys):
+    """The library and the launcher are there, the binding is not, and an older one is taken away."""
+    monkeypatch.setattr(build, "LAUNCHER", tmp_path / "bin" / "klab")
+    monkeypatch.setattr(build, "BINDING", tmp_path / "klab_torch.so")
+    monkeypatch.setattr(build, "OBJ", tmp_path)
+    run, paths = build._run, sysconfig.get_paths()
+    monkeypatch.setattr(build, "_compile", lambda source, headers, verbose=False: source)  # the library is not what this is about
+    monkeypatch.setattr(build, "_run", lambda cmd: None if cmd[0] == build.nvcc() else run(cmd))
+    monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {**paths, "include": str(tmp_path)})
+    build.BINDING.write_bytes(b"of another torch")
+    assert build.build() == build.LIBRARY
+    assert build.LAUNCHER.exists() and not build.BINDING.exists()
+    assert "Python.h" in capsys.readouterr().err

@@ -41,3 +41,23 @@ def test_out_of_memory_is_torchs_error(little_memory, binding, monkeypatch):
         with pytest.raises(torch.OutOfMemoryError):
             call()
     assert not kv_pages.read(buf, slots[:3], 256)[0].any()  # and goes on
+
+
+def test_without_the_binding(monkeypatch, tmp_path):
+    """A build without it (no headers of torch): the same results through ctypes, and a warning once."""
+    from klab_b200 import _launch, kv_pages
+
+    buf = kv_pages.empty_pages(2, 2, 16, 64)
+    k = torch.randn(5, 2, 64, device="cuda").bfloat16()
+    slots = i32([3, 17, -1, 4, 30])
+    kv_pages.store(k, k, buf, slots)
+    want = kv_pages.read(buf, slots, 64)
+    monkeypatch.setattr(_launch, "fast", None)
+    monkeypatch.setattr(_launch, "_ready", set())
+    monkeypatch.setattr(_launch, "BINDING", tmp_path / "klab_torch.so")
+    buf.zero_()
+    with pytest.warns(RuntimeWarning, match="ctypes"):
+        kv_pages.store(k, k, buf, slots)
+    assert _launch.fast is None
+    for got, w in zip(kv_pages.read(buf, slots, 64), want):
+        assert torch.equal(got, w)

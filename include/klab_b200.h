@@ -338,6 +338,12 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
                                const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
                                int tokens, int requests, int width, int num_pages, int page_size, int heads,
                                int kv_heads, int dim, int max_new, float scale, void* stream);
+/* The same for an `out` of any content: rows of no request, and of one whose numbers make no sense, become 0. */
+KLAB_API int klab_kv_attention_new(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
+                                   const int* lengths, const int* starts, void* out, void* scratch,
+                                   long long scratch_bytes, int tokens, int requests, int width, int num_pages,
+                                   int page_size, int heads, int kv_heads, int dim, int max_new, float scale,
+                                   void* stream);
 KLAB_API long long klab_kv_attention_scratch(int requests, int width, int page_size, int heads, int kv_heads, int dim,
                                              int max_new);
 

@@ -29,8 +29,8 @@ _streams = {}
 _ready = set()
 _lock = threading.Lock()
 # The entry points in the order that the binding takes them.
-_ENTRIES = ("klab_kv_build_step", "klab_kv_store", "klab_kv_read", "klab_kv_attention", "klab_kv_attention_scratch",
-            "klab_adapter_linear", "klab_adapter_scratch")
+_ENTRIES = ("klab_kv_build_step", "klab_kv_store", "klab_kv_read", "klab_kv_attention", "klab_kv_attention_new",
+            "klab_kv_attention_scratch", "klab_adapter_linear", "klab_adapter_scratch")
 BINDING = _native.LIB_DIR / "klab_torch.so"
 fast = None  # the binding, once a device is ready
 

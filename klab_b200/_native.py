@@ -62,6 +62,7 @@ _SIGNATURES = {
     "klab_kv_store": (_I, [_P, _P, _I] + [ct.c_longlong] * 4 + [_P, _P] + [_I] * 5 + [_P]),
     "klab_kv_read": (_I, [_P] * 4 + [_I] * 6 + [_P]),
     "klab_kv_attention": (_I, [_P, ct.c_longlong, _I] + [_P] * 6 + [ct.c_longlong] + [_I] * 9 + [ct.c_float, _P]),
+    "klab_kv_attention_new": (_I, [_P, ct.c_longlong, _I] + [_P] * 6 + [ct.c_longlong] + [_I] * 9 + [ct.c_float, _P]),
     "klab_kv_attention_scratch": (ct.c_longlong, [_I] * 7),
     "klab_adapter_linear": (_I, [_I] + [_P] * 8 + [_I] * 6 + [_P, ct.c_longlong, _P, _SZ, _P]),
     "klab_adapter_scratch": (ct.c_longlong, [_I] * 5),

@@ -97,7 +97,7 @@ struct KvAttnParams {
   float* sums;      // [..][dim]
   int* status;
   long long q_stride;
-  int requests, tokens, width, num_pages, page_shift, heads, kv_heads, group, group_div, max_new, max_length, whole;
+  int requests, tokens, width, num_pages, page_shift, heads, kv_heads, group, group_div, max_new, max_length, whole, fill;
   float scale_log2e;
 };
 
@@ -178,7 +178,7 @@ struct Share {
   Request r;
 };
 
-__device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int ctas, bool report) {
+__device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int ctas, bool report, bool& wrong) {
   constexpr int kFlight = 4;  // requests of a lane whose loads are in flight at once
   const int lane = threadIdx.x & 31, each = (p.requests + 31) / 32;
   bool bad = false;
@@ -214,7 +214,8 @@ __device__ __forceinline__ Share find_share(const KvAttnParams& p, int cta, int 
   }
   int upto = scan(mine);
   const int all = __shfl_sync(0xffffffffu, upto, 31);
-  if (__any_sync(0xffffffffu, bad) && report) record_status(p.status, kStatusBadLength);
+  wrong = __any_sync(0xffffffffu, bad);
+  if (wrong && report) record_status(p.status, kStatusBadLength);
   Share it;
   it.request = it.tile = it.unit = it.first = it.last = 0;
   auto take = [&](const Request& r, int from) {
@@ -321,6 +322,28 @@ __device__ __forceinline__ void next_segment(const KvAttnParams& p, Share& it) {
   if (it.r.tiles == 0) it.pos = it.end;  // not with lengths that stay as they are during the call
 }
 
+// Rows of `out` that belong to no request become 0 (this kv head's part, rows dealt to the warps of all CTAs): those before
+// the first request's and behind the last one's, and where a request's numbers make no sense all that no other one has.
+__device__ __noinline__ void fill_rows(const KvAttnParams& p, int first, int last, bool wrong, int kvh, int dim) {
+  const int lane = threadIdx.x & 31, warps = gridDim.x * kWarps;
+  const int count = wrong ? p.tokens : first + p.tokens - last;
+  for (int i = blockIdx.x * kWarps + (threadIdx.x >> 5); i < count; i += warps) {
+    int row = i;
+    if (wrong) {
+      bool held = false, bad = false;
+      for (int r = lane; r < p.requests; r += 32) {
+        const Request q = make_request(p, p.lengths[r], p.starts[r], p.starts[r + 1], bad);
+        held |= q.tiles > 0 && row >= q.token0 && row < q.token0 + q.fresh;
+      }
+      if (__any_sync(0xffffffffu, held)) continue;
+    } else if (i >= first) {
+      row = last + i - first;
+    }
+    uint4* to = reinterpret_cast<uint4*>(p.out + (static_cast<long long>(row) * p.heads + kvh * p.group) * dim);
+    for (int c = lane; c < p.group * dim / 8; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // CTAs per SM the registers are cut for; heads of 256 hold twice the accumulators.
 constexpr int kv_resident(int ng) { return ng <= 4 ? 3 : 2; }
 
@@ -329,7 +352,7 @@ __device__ __forceinline__ long long record_of(const KvAttnParams& p, int cta, i
 }
 
 template <int NG, bool kBf16>
-__global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(const __grid_constant__ KvAttnParams p) {
   constexpr int D = 32 * NG, Q = NG < 4 ? NG : 4, NQ = NG / Q;
   constexpr int kBytes = kv_block_bytes(D);
   extern __shared__ __align__(128) unsigned char smem[];
@@ -343,7 +366,14 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
   grid_dependency_wait();
   grid_launch_dependents();
 
-  Share it = find_share(p, cta, gridDim.x, cta == 0 && kvh == 0 && warp == 0);
+  int before = 0, behind = p.tokens;
+  if (p.fill) {
+    before = min(max(p.starts[0], 0), p.tokens);
+    behind = min(max(p.starts[p.requests], before), p.tokens);
+  }
+  bool wrong;
+  Share it = find_share(p, cta, gridDim.x, cta == 0 && kvh == 0 && warp == 0, wrong);
+  if (p.fill && (wrong || before > 0 || behind < p.tokens)) fill_rows(p, before, behind, wrong, kvh, D);
   if (tid == 0 && kvh == 0) {
     Header h{};
     h.last = -1;
@@ -930,24 +960,10 @@ int dispatch_kv(int dim, const KvAttnParams& p, const KvPlan& plan, cudaStream_t
   }
 }
 
-}  // namespace
-}  // namespace klab
-
-extern "C" {
-
-KLAB_API long long klab_kv_attention_scratch(int requests, int width, int page_size, int heads, int kv_heads, int dim,
-                                             int max_new) {
-  klab::KvPlan plan{};
-  const int rc = klab::kv_plan(requests, width, page_size, heads, kv_heads, dim, max_new, &plan);
-  if (rc) return rc < 0 ? rc : -rc;
-  return static_cast<long long>(plan.total);
-}
-
-KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
-                               const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
-                               int tokens, int requests, int width, int num_pages, int page_size, int heads,
-                               int kv_heads, int dim, int max_new, float scale, void* stream) {
-  using namespace klab;
+int run_attention(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
+                 const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes, int tokens,
+                 int requests, int width, int num_pages, int page_size, int heads, int kv_heads, int dim, int max_new,
+                 float scale, void* stream, bool fill) {
   if (!q || !pages || !table || !lengths || !starts || !out || !scratch || tokens <= 0 || num_pages <= 0)
     return KLAB_E_INVALID;
   if (dtype != KLAB_DT_BF16 && dtype != KLAB_DT_F16) return KLAB_E_UNSUPPORTED;
@@ -985,9 +1001,39 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
   p.max_length = width * page_size;
   p.whole = plan.whole;
   p.max_new = max_new;
+  p.fill = fill;
   p.scale_log2e = scale * 1.44269504088896340736f;
   return dtype == KLAB_DT_BF16 ? dispatch_kv<true>(dim, p, plan, static_cast<cudaStream_t>(stream))
                                : dispatch_kv<false>(dim, p, plan, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace klab
+
+extern "C" {
+
+KLAB_API long long klab_kv_attention_scratch(int requests, int width, int page_size, int heads, int kv_heads, int dim,
+                                             int max_new) {
+  klab::KvPlan plan{};
+  const int rc = klab::kv_plan(requests, width, page_size, heads, kv_heads, dim, max_new, &plan);
+  if (rc) return rc < 0 ? rc : -rc;
+  return static_cast<long long>(plan.total);
+}
+
+KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
+                               const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
+                               int tokens, int requests, int width, int num_pages, int page_size, int heads,
+                               int kv_heads, int dim, int max_new, float scale, void* stream) {
+  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests, width, num_pages,
+                            page_size, heads, kv_heads, dim, max_new, scale, stream, false);
+}
+
+KLAB_API int klab_kv_attention_new(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
+                               const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
+                               int tokens, int requests, int width, int num_pages, int page_size, int heads,
+                               int kv_heads, int dim, int max_new, float scale, void* stream) {
+  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests, width, num_pages,
+                            page_size, heads, kv_heads, dim, max_new, scale, stream, true);
 }
 
 }  // extern "C"

@@ -29,7 +29,7 @@ struct Entries {
   decltype(&klab_kv_build_step) build_step = nullptr;
   decltype(&klab_kv_store) store = nullptr;
   decltype(&klab_kv_read) read = nullptr;
-  decltype(&klab_kv_attention) attention = nullptr;
+  decltype(&klab_kv_attention) attention = nullptr, attention_new = nullptr;
   decltype(&klab_kv_attention_scratch) attention_scratch = nullptr;
   decltype(&klab_adapter_linear) adapter = nullptr;
   decltype(&klab_adapter_scratch) adapter_scratch = nullptr;
@@ -307,10 +307,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor out = given ? *given : empty({tokens, heads, dim}, q->scalar_type(), index);
     const Tensor scratch = empty({need}, at::kByte, index);  // of this call alone
     auto p = [](const Tensor& t) { return static_cast<const int*>(t.data_ptr()); };
-    launch.done(g_entry.attention(q->data_ptr(), stride, type, pages->data_ptr(), p(*table), p(*lengths), p(*starts),
-                                  out.data_ptr(), scratch.data_ptr(), need, i(tokens), i(requests), i(width), i(num),
-                                  i(page_size), i(heads), i(kv_heads), i(dim), i(max_new), static_cast<float>(scale),
-                                  launch.stream()));
+    const auto attend = given ? g_entry.attention : g_entry.attention_new;
+    launch.done(attend(q->data_ptr(), stride, type, pages->data_ptr(), p(*table), p(*lengths), p(*starts), out.data_ptr(),
+                       scratch.data_ptr(), need, i(tokens), i(requests), i(width), i(num), i(page_size), i(heads),
+                       i(kv_heads), i(dim), i(max_new), static_cast<float>(scale), launch.stream()));
     launch.used(*q, *pages, *table, *lengths, *starts);
     if (!given) return THPVariable_Wrap(out);
     launch.used(out);
@@ -388,12 +388,12 @@ PyObject* adapter_linear(PyObject*, PyObject* const* o, Py_ssize_t count) {
 
 // bind(addresses of the entry points, in the order of Entries)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* p[7];
-  if (n != 7) {
-    PyErr_SetString(PyExc_ValueError, "bind takes the addresses of 7 entry points");
+  void* p[8];
+  if (n != 8) {
+    PyErr_SetString(PyExc_ValueError, "bind takes the addresses of 8 entry points");
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i) {
+  for (int i = 0; i < 8; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "an entry point is null");
@@ -404,9 +404,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_entry.store = reinterpret_cast<decltype(g_entry.store)>(p[1]);
   g_entry.read = reinterpret_cast<decltype(g_entry.read)>(p[2]);
   g_entry.attention = reinterpret_cast<decltype(g_entry.attention)>(p[3]);
-  g_entry.attention_scratch = reinterpret_cast<decltype(g_entry.attention_scratch)>(p[4]);
-  g_entry.adapter = reinterpret_cast<decltype(g_entry.adapter)>(p[5]);
-  g_entry.adapter_scratch = reinterpret_cast<decltype(g_entry.adapter_scratch)>(p[6]);
+  g_entry.attention_new = reinterpret_cast<decltype(g_entry.attention_new)>(p[4]);
+  g_entry.attention_scratch = reinterpret_cast<decltype(g_entry.attention_scratch)>(p[5]);
+  g_entry.adapter = reinterpret_cast<decltype(g_entry.adapter)>(p[6]);
+  g_entry.adapter_scratch = reinterpret_cast<decltype(g_entry.adapter_scratch)>(p[7]);
   Py_RETURN_NONE;
 }
 

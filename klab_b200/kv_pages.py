@@ -283,7 +283,8 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
     q [tokens, heads, head_dim] (BF16 or FP16, any token stride that is a multiple of 8 elements): request i's rows are
     starts[i] .. starts[i+1], at most max_new (<= 16) of them, the last of its lengths[i] tokens; token j of n sees positions
     below lengths[i] - n + j + 1, and a row that sees none gives zeros. scale defaults to 1 / sqrt(head_dim). Rows of q
-    that belong to no request leave their rows of `out` as they were.
+    that belong to no request (a padded batch's) leave their rows of a given `out` as they were; in a new result they are
+    zeros.
     """
     if _launch.fast is not None:
         done = _launch.fast.attention(q, pages, table, lengths, starts, max_new, scale, out)
@@ -322,15 +323,15 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
                 or out.data_ptr() % 16 or out.requires_grad:
             raise ValueError("out must be contiguous, 16-byte aligned, of q's shape, dtype and device")
         _disjoint(out, q, pages, table, lengths, starts)
-        tensors = (q, pages, table, lengths, starts, out)
+        name, tensors = "klab_kv_attention", (q, pages, table, lengths, starts, out)
     else:
         out = torch.empty(tokens, heads, dim, device=device, dtype=dtype)
-        tensors = (q, pages, table, lengths, starts)
+        name, tensors = "klab_kv_attention_new", (q, pages, table, lengths, starts)
     index = ready(device)
     # Scratch of this call alone: a captured graph keeps its own, and nothing has to be zero in it.
     need = _scratch_bytes(index, requests, width, page_size, heads, kv_heads, dim, max_new)
     scratch = torch.empty(need, device=device, dtype=torch.uint8)
-    launch("klab_kv_attention", index,
+    launch(name, index,
            (qp, token_stride if tokens > 1 else 0, _DT[dtype], pages.data_ptr(), table.data_ptr(), lengths.data_ptr(),
             starts.data_ptr(), out.data_ptr(), scratch.data_ptr(), need, tokens, requests, width, num_pages, page_size, heads,
             kv_heads, dim, max_new, scale), tensors)

@@ -1,12 +1,12 @@
-"""Attention over 4-bit pages at the ends of its range: one huge value of V, weak values under a long tail, and scores and
-scales near the largest floats."""
+"""Attention over 4-bit pages at the ends of its range: one huge value of V, weak values under a long tail, scores and
+scales near the largest floats, and rows of no request."""
 
 import numpy as np
 import pytest
 import torch
 
 from oracle import kv_pages as ok
-from test_gpu_kv_pages import DT, close, f64, i32, native  # noqa: F401
+from test_gpu_kv_pages import DT, attention_case, close, f64, i32, native  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,65 @@ def test_far_scores_stay_finite(dtype, times, scale):
         assert (np.abs(f64(out)[0] - want) <= (half + 2.0 ** -10) * np.abs(want)).all()
     else:
         close(out, q, [0], [n], [1], k, v, dtype, scale=scale if times else 1.0)
+
+
+@pytest.fixture
+def dirty_memory():
+    """What the allocator gives out next holds NaN."""
+    def spoil(*shape, dtype):
+        torch.cuda.synchronize()
+        for t in [torch.full(shape, float("nan"), device="cuda", dtype=dtype) for _ in range(4)]:
+            del t
+    return spoil
+
+
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("lengths,new,heads,kvh,dim,gap", [([40, 17], [1, 1], 8, 2, 64, 3), ([900, 40, 333], [1, 0, 2], 28, 4, 128, 40),
+                                                           ([0, 0], [0, 0], 4, 4, 256, 5), ([700], [16], 16, 1, 128, 700),
+                                                           ([30] * 70, [1] * 70, 4, 1, 64, 1)])
+def test_rows_of_nobody_are_zeros_in_a_new_result(native, dirty_memory, monkeypatch, binding, lengths, new, heads, kvh, dim, gap):  # noqa: F811
+    """A padded batch's rows, before the first request's and behind the last one's; a request whose numbers make no sense."""
+    from klab_b200 import _launch, kv_pages
+
+    q, buf, table, ln, st, starts, k, v = attention_case(lengths, new, heads, kvh, dim, 16, "bf16", 3, gap=gap)
+    most = max(1, *new)
+    want = torch.full(q.shape, 7.0, device="cuda", dtype=q.dtype)
+    kv_pages.attention(q, buf, table, ln, st, max_new=most, out=want)
+    assert want[starts[-1]:].eq(7.0).all()
+    want[starts[-1]:] = 0
+    if not binding:
+        monkeypatch.setattr(_launch, "fast", None)
+    dirty_memory(*q.shape, dtype=q.dtype)
+    assert torch.equal(kv_pages.attention(q, buf, table, ln, st, max_new=most), want)
+    # The requests begin behind `gap` rows.
+    late = torch.cat([q[starts[-1]:], q[:starts[-1]]])
+    dirty_memory(*q.shape, dtype=q.dtype)
+    got = kv_pages.attention(late, buf, table, ln, st + gap, max_new=most)
+    assert not got[:gap].any() and torch.equal(got[gap:], want[:starts[-1]])
+    if len(lengths) > 1 and new[0]:
+        wrong = ln.clone()
+        wrong[0] = -1
+        dirty_memory(*q.shape, dtype=q.dtype)
+        got = kv_pages.attention(q, buf, table, wrong, st, max_new=most)
+        torch.cuda.synchronize()
+        assert native.device_status(clear=True) == 3
+        assert not got[:new[0]].any() and torch.equal(got[new[0]:], want[new[0]:])
+
+
+def test_rows_of_nobody_in_a_captured_call():
+    """One graph, replayed for fewer and more requests' rows: what an earlier replay left is not there."""
+    from klab_b200 import kv_pages
+
+    q, buf, table, ln, st, starts, k, v = attention_case([50, 60, 70], [1, 1, 1], 8, 2, 64, 16, "fp16", 5, gap=4)
+    kv_pages.attention(q, buf, table, ln, st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kv_pages.attention(q, buf, table, ln, st)
+    graph.replay()
+    whole = out.clone()
+    for rows in (0, 1, 3, 2):
+        st.copy_(i32(np.minimum(np.arange(4), rows)))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:rows], whole[:rows]) and not out[rows:].any()

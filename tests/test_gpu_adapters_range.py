@@ -1,5 +1,7 @@
 """Adapters beside the shared projection: values of x far apart and near the largest, many
-rows, and operands that the launch before wrote."""
+rows, operands that the launch before wrote, operands off 16-byte boundaries, and both ways to launch."""
+
+from dataclasses import replace
 
 import pytest
 import torch
@@ -113,3 +115,74 @@ def test_operands_that_the_launch_before_wrote(kind, captured):
         got = [one(*o) for o in order]
     for v, (i, last) in zip(got, order):
         assert torch.equal(v, want[i]), (i, last)
+
+
+def moved(t, by):
+    """The same values `by` bytes behind a 512-byte boundary."""
+    held = torch.empty(t.numel() * t.element_size() + 64, device="cuda", dtype=torch.uint8)
+    assert held.data_ptr() % 512 == 0
+    out = held[by:by + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("m", [1, 3, 9, 40])
+@pytest.mark.parametrize("kind,k,by", [("bf16", 1000, 4), ("bf16", 512, 8), ("int8", 1000, 0), ("int8", 1024, 4), ("int8", 264, 8),
+                                       ("fp4", 1024, 4), ("fp4", 992, 8), ("fp4", 1024, 12)])
+def test_weights_off_16_byte_boundaries(kind, k, by, m):
+    """Rows or addresses that the streamed form does not take run the projection between the two small kernels."""
+    from klab_b200 import fp4, int8_weights
+    from klab_b200.adapters import adapter_linear
+
+    w, exact, *rest = case(kind, m, 130, k, 16, 3, seed=2)
+    if kind == "bf16":
+        w = moved(w, by)
+    elif kind == "int8":
+        w = int8_weights.Int8Weights(moved(w.codes, by), w.scales)
+    else:
+        w = fp4.FP4F16Weights(moved(w.packed, by), w.scales)
+    for dtype in (torch.bfloat16, torch.float32):
+        close(adapter_linear(rest[0], w, *rest[1:], output_dtype=dtype), exact, *rest, dtype)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp4"])
+def test_scales_off_16_byte_boundaries(kind):
+    from klab_b200.adapters import adapter_linear
+
+    w, exact, *rest = case(kind, 6, 300, 2048, 16, 3, seed=6)
+    want = adapter_linear(rest[0], w, *rest[1:])
+    close(want, exact, *rest, torch.bfloat16)
+    for by in (w.scales.element_size(), 2 * w.scales.element_size()):
+        assert torch.equal(adapter_linear(rest[0], replace(w, scales=moved(w.scales, by)), *rest[1:]), want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp4"])
+@pytest.mark.parametrize("m", [1, 16, 40])
+def test_both_launch_paths_agree(kind, m, monkeypatch):
+    """The binding serves streamed formats; without it the wrapper launches the same kernels through ctypes."""
+    from klab_b200 import _launch
+    from klab_b200.adapters import adapter_linear
+
+    w, _, *rest = case(kind, m, 300, 1024, 16, 3)
+
+    def everything():
+        out = torch.empty(m, 300, device="cuda", dtype=torch.float32)
+        assert adapter_linear(rest[0], w, *rest[1:], out=out, output_dtype=torch.float32) is out
+        return adapter_linear(rest[0], w, *rest[1:]), out
+
+    everything()
+    real, served = _launch.fast, []
+
+    class Counting:
+        def adapter_linear(self, *a):
+            done = real.adapter_linear(*a)
+            served.append(done is not None)
+            return done
+
+    with monkeypatch.context() as patch:
+        patch.setattr(_launch, "fast", Counting())
+        first = everything()
+    assert served == [True, True]
+    monkeypatch.setattr(_launch, "fast", None)
+    for a, b in zip(first, everything()):
+        assert torch.equal(a, b)

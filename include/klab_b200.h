@@ -292,6 +292,12 @@ KLAB_API int klab_decode_attention(const void* q, const void* k_new, const void*
  * request in order. No counterpart in the reference, whose cache is one sequence's (research/l2-prefetch/src/
  * decode_attn.py:20-107). */
 
+/* Limits: requests of a batch, new tokens of a request in one attention call, query heads of a kv head, rank of an adapter. */
+#define KLAB_KV_MAX_REQUESTS 8192
+#define KLAB_KV_MAX_NEW 16
+#define KLAB_KV_MAX_GROUP 64
+#define KLAB_ADAPTER_MAX_RANK 256
+
 /* Results of klab_kv_build_step. */
 #define KLAB_STEP_OK 0
 #define KLAB_STEP_LENGTH 1 /* a negative length or new-token count */

@@ -31,6 +31,7 @@
 #include "common.cuh"
 #include "klab_b200.h"
 #include "klab_kernels.h"
+#include "launch.cuh"
 
 namespace klab {
 namespace {
@@ -38,7 +39,7 @@ namespace {
 constexpr int kAdThreads = 256;
 constexpr int kAdWarps = kAdThreads / 32;
 constexpr int kRanks = 4;  // rows of A per CTA
-constexpr int kMaxRank = 256;
+constexpr int kMaxRank = KLAB_ADAPTER_MAX_RANK;
 
 struct AdapterParams {
   const unsigned short* x;
@@ -657,21 +658,6 @@ size_t plain_scratch(int m, int n, int rank) {
   return plain_t(held, rank) + static_cast<size_t>(held) * n * 4;
 }
 
-template <typename Kernel>
-int launch_stream(Kernel kernel, dim3 grid, int threads, size_t smem, const StreamParams& p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <int KIND, int NB>
 int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
@@ -683,40 +669,9 @@ int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t strea
     if (err != cudaSuccess) return err;
     ready.fetch_or(1ull << dev);
   }
-  const int rc = launch_stream(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, as_smem(KIND), p, stream);
+  const int rc = launch_dependent(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, as_smem(KIND), stream, p);
   if (rc) return rc;
-  return launch_stream(adapter_join_kernel<KIND>, dim3(p.w_blocks, p.m), kAsRows, 0, p,
-                       stream);
-}
-
-int sm_count(int* sms) {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  if (dev < 0 || dev >= 64) return KLAB_E_UNSUPPORTED;
-  int n = cached[dev].load();
-  if (!n) {
-    err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (err != cudaSuccess) return err;
-    cached[dev].store(n);
-  }
-  *sms = n;
-  return 0;
-}
-
-template <typename Kernel>
-int launch_adapter(Kernel kernel, dim3 grid, const AdapterParams& p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kAdThreads);
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return launch_dependent(adapter_join_kernel<KIND>, dim3(p.w_blocks, p.m), kAsRows, 0, stream, p);
 }
 
 }  // namespace
@@ -730,7 +685,7 @@ KLAB_API long long klab_adapter_scratch(int wfmt, int m, int n, int k, int rank)
   size_t need = plain_scratch(m, n, rank);  // streamed formats with rows off 16-byte boundaries too
   int kind = 0, sms = 0;
   if (stream_kind(wfmt, &kind)) {
-    const int rc = sm_count(&sms);
+    const int rc = device_sms(&sms);
     if (rc) return rc < 0 ? rc : -rc;
     const int rows = stream_rows(kind, m, n, k, rank, 2 * sms);
     for (const int part : {rows, m % rows}) {
@@ -765,7 +720,7 @@ KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const v
   int kind = 0;
   if (stream_kind(wfmt, &kind)) {
     int sms = 0;
-    const int rc = sm_count(&sms);
+    const int rc = device_sms(&sms);
     if (rc) return rc;
     const int rows = stream_rows(kind, m, n, k, rank, 2 * sms);
     StreamParams q{};
@@ -825,11 +780,11 @@ KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const v
     p.x = static_cast<const unsigned short*>(x) + static_cast<long long>(m0) * k;
     p.ids = ids + m0;
     p.out = static_cast<unsigned char*>(out) + static_cast<long long>(m0) * n * out_bytes;
-    int rc = launch_adapter(shrink_kernel, dim3(rank / kRanks, p.m), p, s);
+    int rc = launch_dependent(shrink_kernel, dim3(rank / kRanks, p.m), kAdThreads, 0, s, p);
     if (rc) return rc;
     rc = klab_gemv(wfmt, KLAB_DT_BF16, p.x, k, w, aux, nullptr, y0, n, KLAB_DT_F32, p.m, n, k, workspace, workspace_bytes, stream);
     if (rc) return rc;
-    rc = launch_adapter(expand_kernel, dim3((n + kAdThreads - 1) / kAdThreads, p.m), p, s);
+    rc = launch_dependent(expand_kernel, dim3((n + kAdThreads - 1) / kAdThreads, p.m), kAdThreads, 0, s, p);
     if (rc) return rc;
   }
   return 0;

@@ -46,6 +46,7 @@
 #include "klab_b200.h"
 #include "klab_kernels.h"
 #include "kv_pages.cuh"
+#include "launch.cuh"
 
 namespace klab {
 namespace {
@@ -873,29 +874,13 @@ struct KvPlan {
   size_t smem;
 };
 
-int kv_sms(int* sms) {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  if (dev < 0 || dev >= 64) return KLAB_E_UNSUPPORTED;
-  int n = cached[dev].load();
-  if (!n) {
-    err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (err != cudaSuccess) return err;
-    cached[dev].store(n);
-  }
-  *sms = n;
-  return 0;
-}
-
 int kv_plan(int requests, int width, int page_size, int heads, int kv_heads, int dim, int max_new, KvPlan* plan) {
   if (requests <= 0 || width <= 0 || heads <= 0 || kv_heads <= 0 || max_new <= 0) return KLAB_E_INVALID;
-  if (requests > kKvMaxRequests || kv_heads > 65535 || heads % kv_heads || heads / kv_heads > 64 || max_new > kKvMaxNew ||
+  if (requests > kKvMaxRequests || kv_heads > 65535 || heads % kv_heads || heads / kv_heads > KLAB_KV_MAX_GROUP || max_new > kKvMaxNew ||
       !kv_dim_ok(dim) || !kv_page_size_ok(page_size) || static_cast<long long>(width) * page_size > INT_MAX)
     return KLAB_E_SHAPE;
   int sms = 0;
-  const int rc = kv_sms(&sms);
+  const int rc = device_sms(&sms);
   if (rc) return rc;
   const int tiles = (heads / kv_heads * max_new + kRows - 1) / kRows;
   const long long units = (static_cast<long long>(width) * page_size - 1) / kUnitTokens + 1;
@@ -918,21 +903,6 @@ int kv_plan(int requests, int width, int page_size, int heads, int kv_heads, int
   return 0;
 }
 
-template <typename... A>
-int launch_kv(void (*kernel)(A...), dim3 grid, size_t smem, cudaStream_t stream, const KvAttnParams& p) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <int NG, bool kBf16>
 int run_kv(const KvAttnParams& p, const KvPlan& plan, cudaStream_t stream) {
   static std::atomic<unsigned long long> ready{0};
@@ -946,9 +916,9 @@ int run_kv(const KvAttnParams& p, const KvPlan& plan, cudaStream_t stream) {
     ready.fetch_or(1ull << dev);
   }
   const dim3 grid(static_cast<unsigned>(plan.ctas), static_cast<unsigned>(p.kv_heads));
-  int rc = launch_kv(kv_attn_kernel<NG, kBf16>, grid, plan.smem, stream, p);
+  int rc = launch_dependent(kv_attn_kernel<NG, kBf16>, grid, kThreads, plan.smem, stream, p);
   if (rc || !plan.combine) return rc;
-  return launch_kv(kv_combine_kernel<32 * NG, kBf16>, grid, 0, stream, p);
+  return launch_dependent(kv_combine_kernel<32 * NG, kBf16>, grid, kThreads, 0, stream, p);
 }
 
 template <bool kBf16>

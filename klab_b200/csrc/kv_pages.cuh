@@ -17,12 +17,14 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include "klab_b200.h"
+
 namespace klab {
 
 constexpr int kKvGroup = 32;        // dims that share a scale
 constexpr int kKvBlock = 16;        // tokens of a block
-constexpr int kKvMaxRequests = 8192;
-constexpr int kKvMaxNew = 16;       // new tokens a request may have in one attention call
+constexpr int kKvMaxRequests = KLAB_KV_MAX_REQUESTS;
+constexpr int kKvMaxNew = KLAB_KV_MAX_NEW;
 
 __host__ __device__ constexpr int kv_block_bytes(int dim) { return 18 * dim; }
 

@@ -29,6 +29,7 @@
 #include "klab_b200.h"
 #include "klab_kernels.h"
 #include "kv_pages.cuh"
+#include "launch.cuh"
 
 namespace klab {
 namespace {
@@ -495,19 +496,8 @@ int check_pages(const void* pages, const void* slots, int tokens, int num_pages,
   return 0;
 }
 
-template <typename Kernel>
-int launch_rows(Kernel kernel, unsigned threads, unsigned block, const RowParams& p, void* stream) {
-  const unsigned blocks = (threads + block - 1) / block;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(block);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+int launch_rows(void (*kernel)(RowParams), unsigned threads, unsigned block, const RowParams& p, void* stream) {
+  return launch_dependent(kernel, dim3((threads + block - 1) / block), block, 0, stream, p);
 }
 
 // One thread for 8 dims of a token, or for 8 dims of 2 or 4 groups of a pair of tokens.

@@ -21,6 +21,7 @@
 #include "klab_b200.h"
 #include "klab_kernels.h"
 #include "kv_pages.cuh"
+#include "launch.cuh"
 
 namespace klab {
 namespace {
@@ -312,18 +313,8 @@ KLAB_API int klab_kv_release(const unsigned char* ended, int* lengths, int* tabl
   int rc = check_tables(requests, width, num_pages, page_size);
   if (rc) return rc;
   if ((rc = prepare_step_device())) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(1);
-  cfg.blockDim = dim3(kStepThreads);
-  cfg.dynamicSmemBytes = 4 * static_cast<size_t>(requests);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = klab_get_option(KLAB_OPT_PDL) ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, release_kernel, ended, lengths, table, free_pages, free_count,
-                            device_status_address(), requests, width, num_pages, page_size);
+  return launch_dependent(release_kernel, dim3(1), kStepThreads, 4 * static_cast<size_t>(requests), stream, ended, lengths, table,
+                          free_pages, free_count, device_status_address(), requests, width, num_pages, page_size);
 }
 
 }  // extern "C"

@@ -41,7 +41,8 @@ struct Failed {
   int code;
 };
 
-constexpr int kMaxRequests = 8192, kMaxNew = 16, kMaxGroup = 64, kMaxRank = 256;
+constexpr int kMaxRequests = KLAB_KV_MAX_REQUESTS, kMaxNew = KLAB_KV_MAX_NEW, kMaxGroup = KLAB_KV_MAX_GROUP;
+constexpr int kMaxRank = KLAB_ADAPTER_MAX_RANK;
 
 // ---------------------------------------------------------------- arguments
 

@@ -32,6 +32,7 @@ HEAD_DIMS = (64, 128, 256)
 GROUP = 32            # dims that share a scale
 MAX_NEW = 16          # new tokens of a request in one attention call
 MAX_REQUESTS = 8192
+MAX_GROUP = 64        # query heads of a kv head
 STEP_OK, STEP_LENGTH, STEP_TABLE, STEP_PAGES, STEP_TOKENS = range(5)
 _DT = {torch.bfloat16: _native.DT_BF16, torch.float16: _native.DT_F16}
 _ODT = {**_DT, torch.float32: _native.DT_F32}
@@ -301,8 +302,8 @@ def attention(q, pages, table, lengths, starts, *, max_new=1, scale=None, out=No
     if tokens <= 0 or dim_stride != 1 or (heads > 1 and head_stride != dim) or (tokens > 1 and token_stride % 8) or qp % 16 \
             or q.device != device:
         raise ValueError("q needs contiguous heads, a token stride of a multiple of 8 and 16-byte alignment on the pages' device")
-    if heads % kv_heads or heads // kv_heads > 64:
-        raise ValueError("heads must be a multiple of kv_heads, at most 64 each")
+    if heads % kv_heads or heads // kv_heads > MAX_GROUP:
+        raise ValueError(f"heads must be a multiple of kv_heads, at most {MAX_GROUP} each")
     for t in (table, lengths, starts):
         if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device:
             raise ValueError(f"table, lengths and starts must be contiguous int32 tensors on {device}")

@@ -1,8 +1,10 @@
-"""Host side of the batched operators without a GPU: sizes of scratch, and a build where the binding's headers are missing."""
+"""Host side of the batched operators without a GPU: sizes of scratch, a build where the binding's headers are missing,
+and limits that Python and C share."""
 
+import re
 import sysconfig
 
-from klab_b200 import _native, build
+from klab_b200 import _native, adapters, build, kv_pages
 
 
 def test_plain_scratch_stays_small():
@@ -28,3 +30,12 @@ def test_build_without_python_headers(tmp_path, monkeypatch, capsys):
     assert build.build() == build.LIBRARY
     assert build.LAUNCHER.exists() and not build.BINDING.exists()
     assert "Python.h" in capsys.readouterr().err
+
+
+def test_limits_are_the_headers():
+    header = (build.INCLUDE / "klab_b200.h").read_text()
+    limits = {name: int(value) for name, value in re.findall(r"#define KLAB_((?:KV|ADAPTER)_MAX_\w+) (\d+)", header)}
+    assert limits == {"KV_MAX_REQUESTS": kv_pages.MAX_REQUESTS, "KV_MAX_NEW": kv_pages.MAX_NEW,
+                      "KV_MAX_GROUP": kv_pages.MAX_GROUP, "ADAPTER_MAX_RANK": adapters.MAX_RANK}
+    steps = {name: int(value) for name, value in re.findall(r"#define KLAB_STEP_(\w+) (\d+)", header)}
+    assert steps == {name[5:]: getattr(kv_pages, name) for name in dir(kv_pages) if name.startswith("STEP_")}

@@ -357,7 +357,8 @@ KLAB_API long long klab_kv_attention_scratch(int requests, int width, int page_s
  * i = ids[t] (-1: the projection alone; another index outside the adapters counts as -1, device status 6). BF16 x [M,K],
  * a [adapters, rank, K], b [adapters, N, rank], c FP32 [adapters], ids int32 [M]; wfmt BF16, CBF16, I8_ROW, I8_G64 or
  * FP4_G32H with its side data in aux. K % 8 == 0, rank % 8 == 0, rank <= 256; x, a, b and scratch 16-byte aligned.
- * scratch: klab_adapter_scratch bytes (a negative value there is an error code) of any content, for this call alone;
+ * scratch: klab_adapter_scratch bytes (a negative value there is an error code; about 64 MiB at most, or the FP32 sums of
+ * 48 rows where those are more) of any content, for this call alone;
  * workspace as for klab_gemv (BF16, I8_ROW and FP4_G32H with 16-byte aligned rows need none). One rounding to
  * out_dtype (BF16 or FP32). No counterpart in the reference. */
 KLAB_API int klab_adapter_linear(int wfmt, const void* x, const void* w, const void* aux, const void* a, const void* b,

@@ -3,12 +3,12 @@
 // BF16 x, A [S, r, K], B [S, N, r]; W in any format that the projections take with BF16 x and one scale tensor.
 //
 // BF16, INT8 per-row and E2M1/FP16-per-32 weights with 16-byte rows: two launches.
-//   adapter_stream_kernel reads W and the tokens' A once, as one list of work: a block is 128 rows (8 warps x 16 rows) of W,
-//   or 8 groups of 16 rows of the tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or
-//   256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM (a block into
+//   adapter_stream_kernel reads, for each tile of 16 tokens, W once and every token's A (one adapter's again for each of its
+//   tokens, from L2), as one list of work: a block is 128 rows (8 warps x 16 rows) of W, or 8 groups of 16 rows of the
+//   tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or 256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM (a block into
 //   shares of its own where that costs little), so any N and K and any number of adapters keep every SM reading to the
 //   end. A warp copies its units into a ring of its own (cp.async,
-//   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this takes 31.3) and
+//   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this took 31.3) and
 //   multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16 bytes of rows g and
 //   g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies in shared memory in
 //   fragment order. Weights, INT8 codes and E2M1 values are exact in BF16 and meet x as it is, so every product is exact
@@ -21,9 +21,10 @@
 // Other formats: shrink_kernel (t in FP32), the projection as it is with FP32 output, expand_kernel (the sum, one rounding).
 // Either form takes parts of the rows one behind the other where the FP32 sums of all would pass 64 MiB.
 //
-// What bounds it: HBM while the units stream (142 MB in 21 us at M = 16, 14336 -> 4096, rank 64; 31.9 us in all), around
-// it launch, the staging of x (1 to 2.5 us) and the join (3 us). M = 1, 4096 -> 4096 BF16 7.5 us, M = 8, 4096 -> 14336
-// INT8 17.0.
+// What bounds it: BF16 the copies while the units stream (M = 16, 14336 -> 4096, rank 64: 148 MB of W and distinct adapters
+// in 31.8 us, 4.7 TB/s over all; issue slots 36 % busy, warps waiting for data), around it launch, the staging of x and the
+// join (3 us). INT8 and E2M1 are bound by issue too (51 and 55 % busy, the ALU pipe 60 and 48 %): a code costs two
+// instructions on its way to BF16. M = 1, 4096 -> 4096 BF16 7.5 us; M = 8, 4096 -> 14336 INT8 17.1; M = 16 E2M1 25.6.
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -146,7 +147,7 @@ constexpr int kAsTokens = 16;            // tokens of a call's tile
 constexpr int kAsWindow = 32 * 1024;     // x in shared memory
 constexpr int kAsMinShare = 2;           // units of a share: fewer would only add records to join
 // Every block gets CTAs of its own where shares grow by at most so many units: a second piece stages x again and starts its
-// ring anew. M = 4, 1856 -> 1000 BF16 4.7 us (equal shares 6.2), M = 16, 4096 -> 14336 E2M1 27.3 (28.2), M = 8 INT8 17.0
+// ring anew. M = 4, 1856 -> 1000 BF16 4.7 us (equal shares 6.1), M = 16, 4096 -> 14336 E2M1 25.6 (26.3), M = 8 INT8 17.1
 // (17.3); 8 units gain nothing more.
 constexpr int kAsSlack = 4;
 // CTAs to a place from which on blocks are not cut: the last round is then short, and no sums are joined. 4096 -> 14336 BF16,
@@ -157,8 +158,8 @@ constexpr int kAsWaves = 4;
 constexpr size_t kAsScratch = 64ull << 20;
 
 // Bytes of a row in a unit and units of a warp in flight, by the kind of W. Longer runs of a row are better for HBM, shorter
-// units even out short shares: M = 16, 14336 -> 4096 BF16 takes 31.3 us with 256-byte units and 33.4 with 128; M = 8,
-// 4096 -> 14336 INT8 (half the bytes) 17.6 and 16.6.
+// units even out short shares: M = 8, 4096 -> 14336 BF16 takes 23.3 us with 256-byte units and 24.6 with 128 (M = 16,
+// 14336 -> 4096 31.8 and 31.6), the same in INT8 (half the bytes) 17.7 and 17.1.
 __host__ __device__ constexpr int as_unit(int kind) { return kind == AD_BF16 ? 256 : 128; }
 __host__ __device__ constexpr int as_depth(int kind) { return kind == AD_BF16 ? 2 : 3; }
 

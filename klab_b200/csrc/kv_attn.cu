@@ -14,8 +14,8 @@
 // Per unit and warp (two blocks of 16 tokens: K and V codes and scales, one bulk copy of 18 * D bytes each into the
 // warp's ring):
 //   S^T = K Q^T   mma.m16n8k16, A = 16 tokens x 16 dims of codes u as FP16 subnormals (u * 2^-24, exact), B = q in FP16
-//                 times a power of two (its row's maximum in [2^14, 2^15), so nothing that counts is lost); each group of
-//                 32 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
+//                 times a power of two (its row's maximum in [2^14, 2^15): exact down to 2^-32 of the row's largest for BF16,
+//                 2^-29 for FP16; the codes need FP16); each group of 32 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
 //                 more MMA of the scales with the groups' sums of q in two FP16 terms, and starts the sum.
 //   softmax       in base 2 against a reference `ref` of the row that moves only when a score passes it by 2^14, so most
 //                 units need no rescale and no cross-lane maximum; weights and sums in FP32.
@@ -31,11 +31,11 @@
 // Scores beyond a row's last position are -inf before the softmax, and the scales of tokens beyond the request are zeroed,
 // so whatever the allocator left there (NaN scales included) has no part.
 //
-// What bounds it: long caches the warps' own chains (about 490 instructions a warp and unit of 4608 bytes at D = 128, IPC
-// 1.7 with the 12 warps that registers allow, the ALU pipe at 48 %), before HBM: 64 x 8192 tokens, 8 kv heads of 128,
-// 243 MB in 60.6 us, 4.0 TB/s; 1 x 131072, 151 MB in 36.6 us, 4.1 TB/s. Four CTAs an SM (80 registers), more shares than
-// CTAs, the next piece's first copies issued ahead and 16 rows a tile all measured the same or slower. Short ones launch,
-// dependent loads (lengths, table, first block) and the join (2.8 us): 1 x 300 tokens 4.9 us.
+// What bounds it: long caches the warps' own chains (about 610 instructions a warp and unit of 4608 bytes at D = 128, issue
+// slots 56 % busy with the 12 warps that registers allow, the ALU pipe 51 %, tensor cores 31 %), before HBM: 64 x 8192
+// tokens, 8 kv heads of 128, 243 MB in 63.4 us, 3.8 TB/s; 1 x 131072, 151 MB in 38.5 us, 3.9 TB/s. Four CTAs an SM (80
+// registers), more shares than CTAs, the next piece's first copies issued ahead and 16 rows a tile all measured the same or
+// slower. Short ones launch, dependent loads (lengths, table, first block) and the join (2.8 us): 1 x 300 tokens 4.9 us.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -55,19 +55,19 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 8;  // query rows of a tile (the MMA's N)
 // Units of two blocks that a warp's ring holds: a third one takes shared memory and L1 from the third CTA of an SM at heads
-// of 64 and 256 (25.9 us against 33.6, 23.1 against 31.7) and changes heads of 128 by 1 %.
+// of 64 and 256 (26.4 us against 32.3, 22.2 against 29.8) and changes heads of 128 by 1 %.
 constexpr int kSlots = 2;
-// Units a CTA takes at least: short batches pay for the sums that every share leaves (8 x 2048 drafts 13.8 us, with 8 units
-// 15.1; 1 x 2000 tokens 7.7 us, with 2 units 8.3, with 8 units 7.9).
+// Units a CTA takes at least: short batches pay for the sums that every share leaves (1 x 2000 tokens 7.9 us, with 2 units
+// 8.4, with 8 units 8.0).
 constexpr int kMinShare = 4;
 // Up to 64 requests whose equal shares have at most kTry units: every segment gets CTAs of its own where shares of up to
-// kSlack units more allow it, since a CTA's second piece starts and ends like its first: 16 x 4096 tokens 14.0 us, with
-// equal shares 16.6; 32 x 1000 12.4 and 18.3; 8 x 2048 drafts 12.1 and 14.2. Above kTry equal shares are as good or better
-// (32 x 8192 35.4 us; 36.1 with the search), and 8 units of slack leave out little (32 x 4096 25.9 us, 16 units 25.6).
+// kSlack units more allow it, since a CTA's second piece starts and ends like its first: 16 x 4096 tokens 14.4 us, with
+// equal shares 16.8; 32 x 1000 12.7 and 18.3; 8 x 2048 drafts 11.9 and 13.9. Above kTry equal shares are as good or better
+// (32 x 8192 36.6 us, 37.4 with the search; 32 x 4096, just under it, 26.5 and 25.8), and 8 units of slack measure the same.
 constexpr int kTry = 40, kSlack = 16;
 constexpr int kUnitTokens = 2 * kKvBlock;
-// Tables of at most this many units are not cut: 1 x 250 tokens 4.9 us against 6.5 cut, 64 x 512 14.6 against 18.7;
-// 1 x 2000 16.6 us whole and 7.7 cut.
+// Tables of at most this many units are not cut: 1 x 250 tokens 5.1 us against 6.6 cut, 64 x 512 15.1 against 19.2;
+// 1 x 2000 17.0 us whole and 7.9 cut.
 constexpr int kWholeUnits = 16;
 constexpr float kNegInf = -__builtin_huge_valf();
 // A row's weights are 2^(score - ref) with ref = (a score near the largest) - 10 + e, moved when a score passes it by

@@ -14,11 +14,12 @@
 //   words where their slots are a pair (all of a prompt but its ends); other tokens write halves.
 //   Many rows: a thread takes two tokens and 8 dims of each of the 4 groups of a quad (read: 2 at heads of 64): K codes, V codes
 //   of a pair of slots and scales are then whole runs of 16 bytes of a block, and the addresses are worked out once for 128
-//   values. (Single runs are bound by issue slots there: 77 % busy at 30 % of DRAM's rate.)
+//   values. (Single runs are bound by issue slots there.)
 // Read: the inverse, (code - 8) * s in FP32 (exact) and one rounding to the output's type; a slot of -1 gives zeros.
 //
 // What bounds them: few rows launch and three dependent loads; many rows the bytes, 4 in and 1.125 out per pair of values
-// (16384 tokens of 8 heads of 128: store 18.0 us, 4.8 TB/s; read 15.8 us, 5.4 TB/s).
+// (16384 tokens of 8 heads of 128: store 18.0 us, 4.8 TB/s; read 15.8 us, 5.4 TB/s), in store with loads that 16 warps an SM
+// (96 registers) keep too few of in flight, and issue slots 50 % busy.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,9 +37,10 @@ namespace {
 
 constexpr int kStoreThreads = 256, kBulkThreads = 128;
 // 8-dim runs of K (and of V) from which a thread takes runs of Q groups of two tokens. Read: 1024 tokens of 8 heads of 128
-// take 2.6 us either way, 64 take 1.6 us by single runs and 2.3 in bulk, 16384 20.0 and 15.8. Store: 1024 tokens 2.9 us by
-// single runs and 3.1 to 4.4 in bulk, 4096 6.8 and 5.0, 16384 22.6 and 18.0 (24.6 where no two tokens share words of V);
-// heads of 64 only by single runs (16384 tokens 12.3 us and 11.4, but 13.5 and 18.5 where no two tokens share words).
+// take 2.5 us either way, 64 take 1.6 us by single runs and 2.3 in bulk, 16384 18.1 and 14.9. Store, of a prompt: 1024
+// tokens 2.8 us by single runs and 3.0 in bulk, 4096 6.7 and 6.2, 8192 12.0 and 9.2, 16384 22.5 and 17.4; where no two
+// tokens share words of V (one token of each of many requests) 4096 6.4 and 9.4, 16384 22.7 and 24.8; heads of 64 only by
+// single runs (16384 tokens 12.3 us and 11.4, but 13.5 and 18.5 where no two tokens share words).
 constexpr long long kReadBulkRuns = 128 * 1024, kStoreBulkRuns = 512 * 1024;
 
 struct RowParams {

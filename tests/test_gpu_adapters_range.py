@@ -186,3 +186,23 @@ def test_both_launch_paths_agree(kind, m, monkeypatch):
     monkeypatch.setattr(_launch, "fast", None)
     for a, b in zip(first, everything()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("m", [2, 16])
+def test_every_code(m):
+    """All INT8 codes, -128 among them, and all pairs of E2M1 codes."""
+    from klab_b200 import fp4, int8_weights
+    from klab_b200.adapters import adapter_linear
+
+    n, k = 192, 1024
+    _, _, x, a, b, c, ids = case("bf16", m, n, k, 8, 2, seed=9)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    codes = torch.arange(n * k, device="cuda").view(n, k).add(torch.arange(n, device="cuda")[:, None]).sub(128).to(torch.int8)
+    scales = torch.rand(n, generator=gen, device="cuda") * 1e-3 + 1e-3
+    assert codes.unique().numel() == 256
+    y = adapter_linear(x, int8_weights.Int8Weights(codes, scales), a, b, c, ids, output_dtype=torch.float32)
+    close(y, f64(codes) * f64(scales)[:, None], x, a, b, c, ids, torch.float32)
+    packed = (torch.arange(n * k // 2, device="cuda").view(n, k // 2) + torch.arange(n, device="cuda")[:, None] * 7).to(torch.uint8)
+    w = fp4.FP4F16Weights(packed, (torch.rand(n, k // 32, generator=gen, device="cuda") * 0.01 + 0.01).half())
+    assert packed.unique().numel() == 256
+    close(adapter_linear(x, w, a, b, c, ids, output_dtype=torch.float32), f64(w.dequantize()), x, a, b, c, ids, torch.float32)

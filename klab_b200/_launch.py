@@ -60,7 +60,8 @@ def ready(device):
                 fast = load_binding()
             if fast is None:
                 if not _ready:
-                    warnings.warn(f"{BINDING.name} is not built: batched operators launch through ctypes", RuntimeWarning, stacklevel=3)
+                    warnings.warn(f"{BINDING.name} is not built: batched operators launch through ctypes", RuntimeWarning,
+                                  stacklevel=3)
             elif index < 64:
                 fast.mark_ready(index)
             _ready.add(index)

@@ -3,17 +3,17 @@
 // BF16 x, A [S, r, K], B [S, N, r]; W in any format that the projections take with BF16 x and one scale tensor.
 //
 // BF16, INT8 per-row and E2M1/FP16-per-32 weights with 16-byte rows: two launches.
-//   adapter_stream_kernel reads, for each tile of 16 tokens, W once and every token's A (one adapter's again for each of its
-//   tokens, from L2), as one list of work: a block is 128 rows (8 warps x 16 rows) of W, or 8 groups of 16 rows of the
-//   tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or 256 bytes of each of its rows. The units, block by block, are cut into equal shares, two CTAs to an SM (a block into
-//   shares of its own where that costs little), so any N and K and any number of adapters keep every SM reading to the
-//   end. A warp copies its units into a ring of its own (cp.async,
-//   whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where this took 31.3) and
-//   multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16 bytes of rows g and
-//   g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies in shared memory in
-//   fragment order. Weights, INT8 codes and E2M1 values are exact in BF16 and meet x as it is, so every product is exact
-//   whatever else the row holds; E2M1 groups are multiplied by their FP16 scale in FP32. What a share holds of a block goes
-//   to scratch in FP32.
+//   adapter_stream_kernel reads, for each tile of 16 tokens, W once and every token's A (one adapter's again for each of
+//   its tokens, from L2), as one list of work: a block is 128 rows (8 warps x 16 rows) of W, or 8 groups of 16 rows of the
+//   tokens' A (token m's adapter against x, of which column m counts), and a unit is 128 or 256 bytes of each of its rows.
+//   The units, block by block, are cut into equal shares, two CTAs to an SM (a block into shares of its own where that
+//   costs little), so any N and K and any number of adapters keep every SM reading to the end. A warp copies its units into
+//   a ring of its own (cp.async, whole runs of a row at a time: 64-byte runs straight into registers measured 36.9 us where
+//   this took 31.3) and multiplies its 16 rows by up to 16 tokens on mma.m16n8k16 with FP32 sums: lane (g, t) takes 16
+//   bytes of rows g and g + 8 as A fragments (the k slots of an MMA may be any columns as long as x's are the same); x lies
+//   in shared memory in fragment order. Weights, INT8 codes and E2M1 values are exact in BF16 and meet x as it is, so every
+//   product is exact whatever else the row holds; E2M1 groups are multiplied by their FP16 scale in FP32. What a share
+//   holds of a block goes to scratch in FP32.
 //   adapter_join_kernel adds the shares of each block in order, forms t = c (x A^T) the same way, and writes
 //   y + t . B_a[n] with one rounding.
 //   More than 16 rows are tiles of 16 that read W again each, from L2 where it holds it (the projections alone do the same,
@@ -213,8 +213,8 @@ __device__ __forceinline__ void i8_pairs(unsigned w, unsigned& lo, unsigned& hi)
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(__byte_perm(u, 0x37373737u, 0x4342)), "r"(__byte_perm(s, 0x37373737u, 0x4342)));
 }
 
-// E2M1 values J and J + 4 of a word times 2^-24 as a BF16 pair, exact: the code's two exponent bits and one mantissa bit at BF16's lowest
-// exponent bits and highest mantissa bit are the value times 2^-126, BF16 subnormal included.
+// E2M1 values J and J + 4 of a word times 2^-24 as a BF16 pair, exact: the code's two exponent bits and one mantissa bit at
+// BF16's lowest exponent bits and highest mantissa bit are the value times 2^-126, BF16 subnormal included.
 template <int J>
 __device__ __forceinline__ unsigned e2m1_pair(unsigned w) {
   const unsigned size = (J == 0 ? w << 6 : J == 1 ? w << 2 : J == 2 ? w >> 2 : w >> 6) & 0x01c001c0u;
@@ -257,7 +257,8 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
 #pragma unroll
     for (int j = 0; j < 16; j += kRowsAtOnce) {
       const bool there = in && j + sub < rows;
-      copy16((KIND == AD_FP4 ? to ^ ((j & 4) << 4) : to) + j * UNIT, there ? static_cast<const void*>(mine + at + j * row_bytes) : p.x, there);
+      copy16((KIND == AD_FP4 ? to ^ ((j & 4) << 4) : to) + j * UNIT,
+             there ? static_cast<const void*>(mine + at + j * row_bytes) : p.x, there);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
@@ -308,7 +309,7 @@ __device__ __forceinline__ void stream_piece(const StreamParams& p, const unsign
   const int s_end = kUnitSteps * u1;
   for (int s0 = kUnitSteps * u0; s0 < s_end; s0 += kSteps) {
     const int steps = min(kSteps, s_end - s0);
-    // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t) ..
+    // ---- x of the window: piece i of step s of lane (g, t) holds columns COLS s + (INT8: 16 t + 8 i, else 32 i + 8 t)
     __syncthreads();  // the last window is read
     const int pieces = steps * P * NB * 32;
     auto fetch = [&](int i) {
@@ -670,7 +671,8 @@ int run_stream(const StreamParams& p, const StreamPlan& plan, cudaStream_t strea
     if (err != cudaSuccess) return err;
     ready.fetch_or(1ull << dev);
   }
-  const int rc = launch_dependent(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, as_smem(KIND), stream, p);
+  const int rc = launch_dependent(adapter_stream_kernel<KIND, NB>, dim3(plan.ctas, plan.tiles), kAsThreads, as_smem(KIND),
+                                  stream, p);
   if (rc) return rc;
   return launch_dependent(adapter_join_kernel<KIND>, dim3(p.w_blocks, p.m), kAsRows, 0, stream, p);
 }

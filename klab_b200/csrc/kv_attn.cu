@@ -14,8 +14,9 @@
 // Per unit and warp (two blocks of 16 tokens: K and V codes and scales, one bulk copy of 18 * D bytes each into the
 // warp's ring):
 //   S^T = K Q^T   mma.m16n8k16, A = 16 tokens x 16 dims of codes u as FP16 subnormals (u * 2^-24, exact), B = q in FP16
-//                 times a power of two (its row's maximum in [2^14, 2^15): exact down to 2^-32 of the row's largest for BF16,
-//                 2^-29 for FP16; the codes need FP16); each group of 32 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
+//                 times a power of two (its row's maximum in [2^14, 2^15): exact down to 2^-28 of the row's largest for
+//                 BF16 and 2^-25 for FP16, below that off by 2^-35 of it at most; the codes need FP16); each group of 32
+//                 dims is multiplied by the token's scale in FP32. -8 * scale * sum q, which turns u into u - 8, is one
 //                 more MMA of the scales with the groups' sums of q in two FP16 terms, and starts the sum.
 //   softmax       in base 2 against a reference `ref` of the row that moves only when a score passes it by 2^14, so most
 //                 units need no rescale and no cross-lane maximum; weights and sums in FP32.
@@ -457,7 +458,8 @@ __global__ void __launch_bounds__(kThreads, kv_resident(NG)) kv_attn_kernel(cons
     const int ef = max(static_cast<int>(__float_as_uint(top) >> 23), 15);
     const float up = __uint_as_float(static_cast<unsigned>(268 - ef) << 23);  // 2^(141 - ef): the maximum becomes < 2^15
     // At most the largest float: scores that far apart are one-hot at any factor of that size, and 0 stays 0.
-    const float mine_rs = fminf(p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 14) << 23) * 16777216.0f, 3.402823466e38f);
+    const float mine_rs =
+        fminf(p.scale_log2e * __uint_as_float(static_cast<unsigned>(ef - 14) << 23) * 16777216.0f, 3.402823466e38f);
     float c0[NG][2];  // of rows 2 t, 2 t + 1
 #pragma unroll
     for (int G = 0; G < NG; ++G) {
@@ -876,8 +878,9 @@ struct KvPlan {
 
 int kv_plan(int requests, int width, int page_size, int heads, int kv_heads, int dim, int max_new, KvPlan* plan) {
   if (requests <= 0 || width <= 0 || heads <= 0 || kv_heads <= 0 || max_new <= 0) return KLAB_E_INVALID;
-  if (requests > kKvMaxRequests || kv_heads > 65535 || heads % kv_heads || heads / kv_heads > KLAB_KV_MAX_GROUP || max_new > kKvMaxNew ||
-      !kv_dim_ok(dim) || !kv_page_size_ok(page_size) || static_cast<long long>(width) * page_size > INT_MAX)
+  if (requests > kKvMaxRequests || kv_heads > 65535 || heads % kv_heads || heads / kv_heads > KLAB_KV_MAX_GROUP ||
+      max_new > kKvMaxNew || !kv_dim_ok(dim) || !kv_page_size_ok(page_size) ||
+      static_cast<long long>(width) * page_size > INT_MAX)
     return KLAB_E_SHAPE;
   int sms = 0;
   const int rc = device_sms(&sms);
@@ -994,16 +997,16 @@ KLAB_API int klab_kv_attention(const void* q, long long q_stride, int dtype, con
                                const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
                                int tokens, int requests, int width, int num_pages, int page_size, int heads,
                                int kv_heads, int dim, int max_new, float scale, void* stream) {
-  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests, width, num_pages,
-                            page_size, heads, kv_heads, dim, max_new, scale, stream, false);
+  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests,
+                             width, num_pages, page_size, heads, kv_heads, dim, max_new, scale, stream, false);
 }
 
 KLAB_API int klab_kv_attention_new(const void* q, long long q_stride, int dtype, const void* pages, const int* table,
                                const int* lengths, const int* starts, void* out, void* scratch, long long scratch_bytes,
                                int tokens, int requests, int width, int num_pages, int page_size, int heads,
                                int kv_heads, int dim, int max_new, float scale, void* stream) {
-  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests, width, num_pages,
-                            page_size, heads, kv_heads, dim, max_new, scale, stream, true);
+  return klab::run_attention(q, q_stride, dtype, pages, table, lengths, starts, out, scratch, scratch_bytes, tokens, requests,
+                             width, num_pages, page_size, heads, kv_heads, dim, max_new, scale, stream, true);
 }
 
 }  // extern "C"
